@@ -226,6 +226,21 @@ int pq_validate_quantize_groups(const void *k, const int64_t *k_strides, int dty
                                 const void *tscale, const void *tmn,
                                 int out_group_capacity, int out_group_offset);
 
+/* The same into the pages of a paged cache (no reference counterpart): of each sequence, the keys of its open pages that are
+ * full become codes and constants of its next sealed pages.  layout, pages [B, W], open_pages [B, Wo], n_sealed [B] (null: none
+ * is sealed) and kv_len [B] as polarquant_paged.h describes them: with j counting from 0, open page j of sequence b is
+ * quantized if n_sealed[b] + j < kv_len[b] / 128, from physical page open_pages[b, j] of keys to physical page
+ * pages[b, n_sealed[b] + j] of codes, where both exist.  Neither counts nor tables are changed.  flags as above, without
+ * PQ_ANGLE_UNIFORM. */
+int pq_seal_pages(const void *keys, const int64_t *layout, uint8_t *codes, void *rscale, void *rmn, void *tscale, void *tmn,
+                  const int32_t *kv_len, const int32_t *n_sealed, const int32_t *pages, const int32_t *open_pages, int W, int Wo,
+                  int B, int Nk, int rbits, int tbits, int dtype, unsigned flags, void *stream);
+
+int pq_validate_seal_pages(const void *keys, const int64_t *layout, const uint8_t *codes, const void *rscale, const void *rmn,
+                           const void *tscale, const void *tmn, const int32_t *kv_len, const int32_t *n_sealed,
+                           const int32_t *pages, const int32_t *open_pages, int W, int Wo, int B, int Nk, int rbits, int tbits,
+                           int dtype, unsigned flags);
+
 /* Device self-test of the quantizer's arithmetic (no reference counterpart).
  * The kernel takes a cheap arctangent / square root first and the exact,
  * eager-torch-identical routines only near a rounding boundary; this runs both on

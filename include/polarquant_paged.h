@@ -1,0 +1,93 @@
+/* polarquant_paged.h — C ABI of libpolarquant_paged.so (gfx950): a paged polar key cache, rows into its pages,
+ * attention of new tokens over them, the weight of each page, and pages out of the tables (no reference counterpart:
+ * the reference keeps one contiguous cache and takes one new token at a time, models/modeling_llama_polar.py:61-101).
+ * Conventions, dtypes and status codes are polarquant.h's: device pointers, a hipStream_t, nothing allocated, no
+ * synchronisation.  float16 or bfloat16, head_dim 128, any grouping of N query heads over Nk KV heads, rbits + tbits <= 8.
+ *
+ * A page holds PQ_PAGE = 128 tokens of every KV head; its parts are addressed by physical page and head:
+ *   keys    half-precision rows [128, 128] of an open page
+ *   values  half-precision rows [128, 128] of any page
+ *   codes   [128, 64] (or packed, [128, 48]) of a sealed page, and rscale, rmn, tscale, tmn [64], as
+ *           pq_quantize_groups makes them
+ * `layout` holds 11 numbers: strides in elements between pages and between heads of keys, values, codes and the
+ * constants (8 numbers), then how many physical pages keys, values and codes have.  Page strides and head strides are
+ * multiples of 8 elements (codes: 16 bytes).
+ * Sequence b's tokens fill its logical pages 0, 1, ..: the first n_sealed[b] are sealed, those behind them open.
+ *   pages [B, W]        physical page of codes and constants of logical page j
+ *   value_pages [B, W]  that of its values
+ *   open_pages [B, Wo]  that of the keys of logical page n_sealed[b] + j
+ * A physical page outside of its pool (-1, say) does not exist: its tokens are not attended to, nothing is written.
+ * The call's tokens are the last of their sequences, packed: sequence b's are rows q_start[b] .. q_start[b + 1] - 1 of T,
+ * at most max_q of them, and it holds kv_len[b] <= max_kv tokens with them.  These counts live on the device; larger ones
+ * are cut to max_q and max_kv (max_kv <= 128 W).  Rows from q_start[B] on are neither read nor written.
+ *
+ * pq_paged_append: q, k, v rows [T, heads * 128] (row strides multiples of 8), each query and key normed over its 128
+ *   channels where q_norm, k_norm [128] are given (x * rsqrt(mean x^2 + eps) * w), then rotated by row positions[t] (null:
+ *   the token's place in its sequence; the nearest row beyond the table) of cos, sin [angle_rows, 128], halves d and
+ *   d + 64 paired; in float32, rounded once.  Queries to q_out [T, N, 128], keys to their open pages (a token in a sealed
+ *   page: nowhere), values to theirs.
+ * pq_paged_attn: out[t, h] = sum_j w_j v_j / sum_j w_j, w_j = exp(scale q . k_j), over the keys j of the sequence up to
+ *   the token's own whose page exists and whose mask[b * mask_row + j] is not 0; zeros where there are none.  lse (or
+ *   null): [T, N] natural logarithm of the sum, -inf where there are none.  Cut into n_splits slices at most
+ *   (pq_paged_attn_plan) through `workspace`.
+ * pq_paged_weights: weights[b, g, j] = onto[b, g, j] (null: 0) + sum over the rows, the query heads of KV head g and the
+ *   keys of page j that the row sees of exp(scale q . k - lse).  (No values are read: their page exists if it is not
+ *   negative.)
+ * pq_evict_pages: of more than `keep` sealed pages those stay that are the first `sinks`, or else have the largest sum
+ *   over the KV heads of weights [B, Nk, W], the earlier of equals; tables and weights close up in order, -1 and 0 behind
+ *   what is left, evicted pages go to freed [B, W] in order, -1 behind them.  W <= PQ_EVICT_MAX_PAGES.
+ */
+#ifndef POLARQUANT_PAGED_H
+#define POLARQUANT_PAGED_H
+
+#include "polarquant.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+#define PQ_PAGE 128
+#define PQ_EVICT_MAX_PAGES 16384
+
+int pq_validate_paged_append(const void *q, int64_t q_row, const void *k, int64_t k_row, const void *v, int64_t v_row, const void *cos, const void *sin,
+                             int64_t angle_rows, const int32_t *positions, const void *q_norm, const void *k_norm, const void *q_out, const void *keys,
+                             const void *values, const int64_t *layout, const int32_t *q_start, const int32_t *kv_len, const int32_t *n_sealed,
+                             const int32_t *value_pages, const int32_t *open_pages, int W, int Wo, int T, int B, int N, int Nk, int max_q, int max_kv, int dtype);
+int pq_paged_append(const void *q, int64_t q_row, const void *k, int64_t k_row, const void *v, int64_t v_row, const void *cos, const void *sin,
+                    int64_t angle_rows, const int32_t *positions, const void *q_norm, const void *k_norm, float eps, void *q_out, void *keys, void *values,
+                    const int64_t *layout, const int32_t *q_start, const int32_t *kv_len, const int32_t *n_sealed, const int32_t *value_pages,
+                    const int32_t *open_pages, int W, int Wo, int T, int B, int N, int Nk, int max_q, int max_kv, int dtype, void *stream);
+
+int pq_paged_attn_plan(int B, int N, int Nk, int max_q, int max_kv, int n_cus);
+size_t pq_paged_attn_workspace_bytes(int T, int N, int n_splits);
+int pq_validate_paged_attn(const void *q, int64_t q_row, const void *keys, const void *values, const uint8_t *codes, const void *rscale, const void *rmn,
+                           const void *tscale, const void *tmn, const int64_t *layout, const int32_t *q_start, const int32_t *kv_len, const int32_t *n_sealed,
+                           const int32_t *pages, const int32_t *value_pages, const int32_t *open_pages, int W, int Wo, const uint8_t *mask, int64_t mask_row,
+                           const void *out, const float *lse, int T, int B, int N, int Nk, int max_q, int max_kv, int rbits, int tbits, int n_splits,
+                           const void *workspace, size_t workspace_bytes, int dtype, unsigned flags);
+int pq_paged_attn(const void *q, int64_t q_row, const void *keys, const void *values, const uint8_t *codes, const void *rscale, const void *rmn,
+                  const void *tscale, const void *tmn, const int64_t *layout, const int32_t *q_start, const int32_t *kv_len, const int32_t *n_sealed,
+                  const int32_t *pages, const int32_t *value_pages, const int32_t *open_pages, int W, int Wo, const uint8_t *mask, int64_t mask_row, void *out,
+                  float *lse, int T, int B, int N, int Nk, int max_q, int max_kv, int rbits, int tbits, float scale, int n_splits, int n_cus, void *workspace,
+                  size_t workspace_bytes, int dtype, unsigned flags, void *stream);
+
+int pq_validate_paged_weights(const void *q, int64_t q_row, const float *lse, const void *keys, const uint8_t *codes, const void *rscale, const void *rmn,
+                              const void *tscale, const void *tmn, const int64_t *layout, const int32_t *q_start, const int32_t *kv_len,
+                              const int32_t *n_sealed, const int32_t *pages, const int32_t *value_pages, const int32_t *open_pages, int W, int Wo,
+                              const uint8_t *mask, int64_t mask_row, const float *onto, const float *weights, int T, int B, int N, int Nk, int max_q,
+                              int max_kv, int rbits, int tbits, int dtype, unsigned flags);
+int pq_paged_weights(const void *q, int64_t q_row, const float *lse, const void *keys, const uint8_t *codes, const void *rscale, const void *rmn,
+                     const void *tscale, const void *tmn, const int64_t *layout, const int32_t *q_start, const int32_t *kv_len, const int32_t *n_sealed,
+                     const int32_t *pages, const int32_t *value_pages, const int32_t *open_pages, int W, int Wo, const uint8_t *mask, int64_t mask_row,
+                     const float *onto, float *weights, int T, int B, int N, int Nk, int max_q, int max_kv, int rbits, int tbits, float scale, int dtype,
+                     unsigned flags, void *stream);
+
+int pq_validate_evict_pages(const float *weights, const int32_t *pages, const int32_t *n_sealed, const int32_t *kv_len, int B, int Nk, int W, int keep, int sinks,
+                            const int32_t *pages_out, const int32_t *n_sealed_out, const int32_t *kv_len_out, const float *weights_out, const int32_t *freed);
+int pq_evict_pages(const float *weights, const int32_t *pages, const int32_t *n_sealed, const int32_t *kv_len, int B, int Nk, int W, int keep, int sinks,
+                   int32_t *pages_out, int32_t *n_sealed_out, int32_t *kv_len_out, float *weights_out, int32_t *freed, void *stream);
+
+#ifdef __cplusplus
+}
+#endif
+#endif /* POLARQUANT_PAGED_H */

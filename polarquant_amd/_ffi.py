@@ -46,6 +46,8 @@ SIGNATURES = {
                            + [c_void_p] * 5 + [c_int, c_int, c_void_p]),
     "pq_validate_quantize_groups": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_uint]
                                     + [c_void_p] * 5 + [c_int, c_int]),
+    "pq_seal_pages": (c_int, [c_void_p] * 11 + [c_int] * 7 + [c_uint, c_void_p]),
+    "pq_validate_seal_pages": (c_int, [c_void_p] * 11 + [c_int] * 7 + [c_uint]),
     "pq_selftest_quantizer_math": (c_int, [c_int, c_void_p, c_void_p]),
     "pq_decode_attn": (c_int, [c_void_p] * 6 + [c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p,
                                                 c_void_p, c_int64, c_void_p, c_int64, c_float]
@@ -171,6 +173,27 @@ RECURRENT_SIGNATURES = {
 }
 
 
+# the paged polar key cache (include/polarquant_paged.h)
+PQ_EVICT_MAX_PAGES = 16384
+PAGED_LIB_PATH = os.path.join(HERE, "libpolarquant_paged.so")
+_ROWS = [c_void_p, c_int64] * 3 + [c_void_p] * 2 + [c_int64] + [c_void_p] * 3
+_TABLES = [c_void_p] * 6 + [c_int] * 2                  # counts and pages, widths
+PAGED_SIGNATURES = {
+    "pq_validate_paged_append": (c_int, _ROWS + [c_void_p] * 4 + [c_void_p] * 5 + [c_int] * 9),
+    "pq_paged_append": (c_int, _ROWS + [c_float] + [c_void_p] * 4 + [c_void_p] * 5 + [c_int] * 9 + [c_void_p]),
+    "pq_paged_attn_plan": (c_int, [c_int] * 6),
+    "pq_paged_attn_workspace_bytes": (c_size_t, [c_int] * 3),
+    "pq_validate_paged_attn": (c_int, [c_void_p, c_int64] + [c_void_p] * 8 + _TABLES + [c_void_p, c_int64, c_void_p, c_void_p] + [c_int] * 9
+                               + [c_void_p, c_size_t, c_int, c_uint]),
+    "pq_paged_attn": (c_int, [c_void_p, c_int64] + [c_void_p] * 8 + _TABLES + [c_void_p, c_int64, c_void_p, c_void_p] + [c_int] * 8 + [c_float, c_int, c_int]
+                      + [c_void_p, c_size_t, c_int, c_uint, c_void_p]),
+    "pq_validate_paged_weights": (c_int, [c_void_p, c_int64] + [c_void_p] * 8 + _TABLES + [c_void_p, c_int64, c_void_p, c_void_p] + [c_int] * 9 + [c_uint]),
+    "pq_paged_weights": (c_int, [c_void_p, c_int64] + [c_void_p] * 8 + _TABLES + [c_void_p, c_int64, c_void_p, c_void_p] + [c_int] * 8 + [c_float, c_int, c_uint, c_void_p]),
+    "pq_validate_evict_pages": (c_int, [c_void_p] * 4 + [c_int] * 5 + [c_void_p] * 5),
+    "pq_evict_pages": (c_int, [c_void_p] * 4 + [c_int] * 5 + [c_void_p] * 6),
+}
+
+
 class PolarQuantError(RuntimeError):
     def __init__(self, status: int, where: str):
         self.status = status
@@ -244,6 +267,11 @@ def latent_lib() -> ctypes.CDLL:
 def recurrent_lib() -> ctypes.CDLL:
     """The library of windowed attention and recurrent mixers."""
     return _load(RECURRENT_LIB_PATH, RECURRENT_SIGNATURES)
+
+
+def paged_lib() -> ctypes.CDLL:
+    """The paged cache's library."""
+    return _load(PAGED_LIB_PATH, PAGED_SIGNATURES)
 
 
 def bench_lib() -> ctypes.CDLL:

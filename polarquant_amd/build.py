@@ -1,7 +1,7 @@
 """Build recipe of the HIP library: hipcc for gfx950, in-tree.
 
     python -m polarquant_amd.build                    # (re)build polarquant_amd/libpolarquant_hip.so, its test build and libpolarquant_bench.so
-    python -m polarquant_amd.build --layers [steps] [latent] [recurrent]   # those libraries alone
+    python -m polarquant_amd.build --layers [steps] [latent] [recurrent] [paged]   # those libraries alone
     python -m polarquant_amd.build --calls            # the builtins through which the wrappers call them (_calls.so) alone
     python -m polarquant_amd.build --phase-timers     # the measuring build (benchmarks/phase_timing.py)
     python -m polarquant_amd.build --probe no_values  # a probe build (benchmarks/probe_bench.py)
@@ -30,13 +30,14 @@ UNITS = [("pq_attn.hip", ("PQ_DTYPE=0",), ".f16"), ("pq_attn.hip", ("PQ_DTYPE=1"
          ("pq_scores.hip", (), ""), ("pq_quantize.hip", (), ""), ("pq_linear.hip", (), ""), ("pq_attn_common.hip", (), ""),
          ("pq_capi.hip", (), ""), ("pq_values.hip", (), ""), ("pq_decode_ops.hip", (), ""), ("pq_prompt_attn.hip", (), "")]
 SOURCES = sorted({u[0] for u in UNITS})
-# libraries of their own, so that a model builds only what it runs: the steps between mixers and matrix products, and the
-# kernels of the mixers by family
+# libraries of their own, so that a model builds only what it runs: the steps between mixers and matrix products, the
+# kernels of the mixers by family, and those of the paged cache
 LAYER_UNITS = {
     "steps": [("pq_steps.hip", (), ""), ("pq_head_linear.hip", (), ""), ("pq_steps_capi.hip", (), "")],
     "latent": [("pq_latent_attn.hip", (), ""), ("pq_latent_norm.hip", (), ""), ("pq_latent_capi.hip", (), "")],
     "recurrent": [("pq_window_attn.hip", (), ""), ("pq_recurrent_chunk.hip", (), ""), ("pq_recurrent.hip", (), ""), ("pq_recurrent_token.hip", (), ""),
                   ("pq_recurrent_capi.hip", (), "")],
+    "paged": [("pq_paged_token.hip", (), ""), ("pq_paged_weights.hip", (), ""), ("pq_paged_rows.hip", (), ""), ("pq_paged_capi.hip", (), "")],
 }
 LAYER_LIBS = {name: os.path.join(HERE, "libpolarquant_%s.so" % name) for name in LAYER_UNITS}
 # measurement aids (a plain streaming read, the attention kernel's loads without its arithmetic): a library of

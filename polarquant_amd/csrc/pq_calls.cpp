@@ -19,6 +19,7 @@
 
 #include "../../include/polarquant.h"
 #include "../../include/polarquant_latent.h"
+#include "../../include/polarquant_paged.h"
 #include "../../include/polarquant_recurrent.h"
 #include "../../include/polarquant_steps.h"
 
@@ -168,7 +169,8 @@ struct Call<R(A...), STRIDES> {
     X(pq_latent_prefill_takes) X(pq_latent_prefill) X(pq_qk_norm) X(pq_ring_append) X(pq_window_plan) X(pq_window_workspace_bytes)         \
     X(pq_window_attn) X(pq_delta_prep) X(pq_scan_workspace_bytes) X(pq_delta_scan) X(pq_memory_gates) X(pq_memory_scan)                    \
     X(pq_head_norm_gate) X(pq_validate_delta_token) X(pq_delta_token) X(pq_validate_memory_token) X(pq_memory_token)        \
-    X(pq_validate_linear_gelu) X(pq_linear_gelu) X(pq_linear_residual) X(pq_gated_normed) X(pq_qkv_rope_append_normed)
+    X(pq_validate_linear_gelu) X(pq_linear_gelu) X(pq_linear_residual) X(pq_gated_normed) X(pq_qkv_rope_append_normed)    \
+    S(pq_seal_pages) S(pq_paged_append) X(pq_paged_attn_plan) X(pq_paged_attn_workspace_bytes) S(pq_paged_attn) S(pq_paged_weights) X(pq_evict_pages)
 
 // A prototype as ctypes writes types: the result's letter, then the parameters'.
 template <typename T>

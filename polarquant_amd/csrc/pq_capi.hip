@@ -132,6 +132,36 @@ int pq_quantize_groups(const void* k, const int64_t* k_strides, int dtype,
     return err == 0 ? PQ_OK : PQ_ERR_LAUNCH;
 }
 
+int pq_validate_seal_pages(const void* keys, const int64_t* layout, const uint8_t* codes, const void* rscale, const void* rmn, const void* tscale,
+                           const void* tmn, const int32_t* kv_len, const int32_t* n_sealed, const int32_t* pages, const int32_t* open_pages, int W, int Wo, int B,
+                           int Nk, int rbits, int tbits, int dtype, unsigned flags) {
+    if (!keys || !layout || !codes || !rscale || !rmn || !tscale || !tmn || !kv_len || !pages || !open_pages) return PQ_ERR_NULL_POINTER;
+    if (B <= 0 || Nk <= 0 || static_cast<long long>(B) * Nk > 65535 || W <= 0 || Wo <= 0) return PQ_ERR_BAD_SHAPE;
+    if (int rc = check_bits(rbits, tbits)) return rc;
+    if (dtype != PQ_F16 && dtype != PQ_BF16) return PQ_ERR_BAD_DTYPE;
+    if (flags & ~static_cast<unsigned>(PQ_WRAP_FP32 | PQ_CODES_PACKED6 | PQ_DEVICE_ATAN2)) return PQ_ERR_BAD_SHAPE;
+    if ((flags & PQ_CODES_PACKED6) && (tbits != 3 || rbits + tbits > 6)) return PQ_ERR_BAD_BITS;
+    for (int i : {0, 1, 4, 5, 6, 7})
+        if (layout[i] < 0 || layout[i] % (i == 4 || i == 5 ? 16 : 8)) return PQ_ERR_BAD_STRIDE;
+    for (int i : {8, 10})
+        if (layout[i] < 0 || layout[i] > INT32_MAX) return PQ_ERR_BAD_SHAPE;
+    if (!aligned(keys, 16) || !aligned(codes, 16) || !aligned(rscale, 16) || !aligned(rmn, 16) || !aligned(tscale, 16) || !aligned(tmn, 16) ||
+        !aligned(kv_len, 4) || !aligned(n_sealed, 4) || !aligned(pages, 4) || !aligned(open_pages, 4))
+        return PQ_ERR_MISALIGNED;
+    return PQ_OK;
+}
+
+int pq_seal_pages(const void* keys, const int64_t* layout, uint8_t* codes, void* rscale, void* rmn, void* tscale, void* tmn, const int32_t* kv_len,
+                  const int32_t* n_sealed, const int32_t* pages, const int32_t* open_pages, int W, int Wo, int B, int Nk, int rbits, int tbits, int dtype,
+                  unsigned flags, void* stream) {
+    if (int rc = pq_validate_seal_pages(keys, layout, codes, rscale, rmn, tscale, tmn, kv_len, n_sealed, pages, open_pages, W, Wo, B, Nk, rbits, tbits, dtype, flags))
+        return rc;
+    const pq::SealPages p{kv_len, n_sealed, pages, open_pages, W, Wo, static_cast<int>(layout[8]), static_cast<int>(layout[10]),
+                          layout[0], layout[1], layout[4], layout[5], layout[6], layout[7]};
+    const int err = pq::launch_seal_pages(keys, p, dtype, B, Nk, rbits, tbits, flags, codes, rscale, rmn, tscale, tmn, static_cast<hipStream_t>(stream));
+    return err == 0 ? PQ_OK : PQ_ERR_LAUNCH;
+}
+
 }  // extern "C"
 
 extern "C" {

@@ -10,6 +10,15 @@ namespace pq {
 int launch_scores(const void* q, const uint8_t* codes, const void* rscale, const void* rmn, const void* tscale,
                   const void* tmn, float* out, int B, int N, int Nk, int Nb, int tbits, int dtype, bool packed6, hipStream_t st);
 
+// Keys of full open pages to the codes of their sequences' next sealed ones (pq_seal_pages): strides in elements between pages and heads.
+struct SealPages {
+    const int32_t *kv_len, *n_sealed, *pages, *open_pages;
+    int W, Wo, n_open, n_pages;
+    int64_t key_page, key_head, code_page, code_head, meta_page, meta_head;
+};
+int launch_seal_pages(const void* keys, const SealPages& pages, int dtype, int B, int Nk, int rbits, int tbits, unsigned flags, uint8_t* codes, void* rscale,
+                      void* rmn, void* tscale, void* tmn, hipStream_t st);
+
 int launch_quantize(const void* k, const int64_t* strides, int dtype, int B, int Nk, int Nb, int rbits, int tbits,
                     unsigned flags, uint8_t* codes, void* rscale, void* rmn, void* tscale, void* tmn,
                     int cap, int off, hipStream_t st);

@@ -34,6 +34,24 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNone = -1.0e30f;         // running maximum before any key
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// the larger of lanes l and l ^ 32, by an exchange of half wavefronts that stays in the vector unit
+__device__ __forceinline__ float both_halves_max(float v) {
+    typedef unsigned int uint2_x __attribute__((ext_vector_type(2)));
+    const uint2_x r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r.x), __uint_as_float(r.y));
+}
+
+typedef float floatx2_a __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2_a __attribute__((ext_vector_type(2)));
+typedef _Float16 halfx2_a __attribute__((ext_vector_type(2)));
+template <typename T> __device__ __forceinline__ uint32_t pack_pair(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack_pair<BF16>(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(floatx2_a{a, b}, bf16x2_a));
+}
+template <> __device__ __forceinline__ uint32_t pack_pair<F16>(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(floatx2_a{a, b}, halfx2_a));
+}
+
 template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return static_cast<uint32_t>(f2lo<T>(a)) | (static_cast<uint32_t>(f2lo<T>(b)) << 16);
 }

@@ -1,0 +1,234 @@
+// C ABI of the paged cache's kernels: host-side argument checks, then the launchers.
+#include "../../include/polarquant_paged.h"
+#include "../../include/polarquant_steps.h"
+#include "pq_paged_internal.h"
+#include "pq_paged_rules.h"
+#include "pq_capi_checks.h"
+
+using namespace pq::capi;
+
+namespace {
+
+bool half_dtype(int d) { return d == PQ_F16 || d == PQ_BF16; }
+
+int check_counts(const int32_t* q_start, const int32_t* kv_len, const int32_t* n_sealed, int W, int Wo, int T, int B, int N, int Nk, int max_q, int max_kv) {
+    if (!q_start || !kv_len) return PQ_ERR_NULL_POINTER;
+    if (int rc = check_tokens(1, T)) return rc;
+    if (B < 1 || B > 65535 || N < 1 || Nk < 1 || N > 65535 || N % Nk != 0 || max_q < 1 || max_q > T || max_kv < 1 || W < 1 || Wo < 0) return PQ_ERR_BAD_SHAPE;
+    if (max_kv > kMaxTokens || static_cast<int64_t>(max_kv) > static_cast<int64_t>(W) * PQ_PAGE || static_cast<int64_t>(T) * N >= (int64_t{1} << 31))
+        return PQ_ERR_BAD_SHAPE;
+    if (!aligned(q_start, 4) || !aligned(kv_len, 4) || !aligned(n_sealed, 4)) return PQ_ERR_MISALIGNED;
+    return PQ_OK;
+}
+
+// strides and page counts of a pool; `codes` may be null
+int check_layout(const int64_t* layout, const void* keys, const void* values, const void* codes, const void* rscale, const void* rmn, const void* tscale,
+                 const void* tmn) {
+    if (!layout || !keys || !values || (codes && (!rscale || !rmn || !tscale || !tmn))) return PQ_ERR_NULL_POINTER;
+    for (int i = 0; i < 8; i++)
+        if (layout[i] < 0 || layout[i] % (i == 4 || i == 5 ? 16 : 8)) return PQ_ERR_BAD_STRIDE;
+    for (int i = 8; i < 11; i++)
+        if (layout[i] < 0 || layout[i] > INT32_MAX) return PQ_ERR_BAD_SHAPE;
+    if (!aligned(keys, 16) || !aligned(values, 16) || !aligned(codes, 16) || !aligned(rscale, 16) || !aligned(rmn, 16) || !aligned(tscale, 16) || !aligned(tmn, 16))
+        return PQ_ERR_MISALIGNED;
+    return PQ_OK;
+}
+
+int check_pages(const void* codes, const int32_t* pages, const int32_t* value_pages, const int32_t* open_pages, int Wo, int rbits, int tbits, unsigned flags) {
+    if (!value_pages || (codes && !pages) || (Wo > 0 && !open_pages)) return PQ_ERR_NULL_POINTER;
+    if (!aligned(pages, 4) || !aligned(value_pages, 4) || !aligned(open_pages, 4)) return PQ_ERR_MISALIGNED;
+    if (flags & ~PQ_CODES_PACKED6) return PQ_ERR_BAD_SHAPE;
+    if (rbits < 1 || tbits < 1 || rbits + tbits > 8 || tbits > PQ_MAX_TBITS) return PQ_ERR_BAD_BITS;
+    if ((flags & PQ_CODES_PACKED6) && (tbits != 3 || rbits + tbits > 6)) return PQ_ERR_BAD_BITS;
+    return PQ_OK;
+}
+
+int check_queries(const void* q, int64_t q_row, int heads, int64_t tokens) {
+    if (!q) return PQ_ERR_NULL_POINTER;
+    if (q_row % 8 || q_row < 0 || q_row > (1 << 24) || (tokens > 1 && q_row < static_cast<int64_t>(heads) * PQ_HEAD_DIM)) return PQ_ERR_BAD_STRIDE;
+    return aligned(q, 16) ? PQ_OK : PQ_ERR_MISALIGNED;
+}
+
+int check_mask(const uint8_t* mask, int64_t mask_row, int B, int max_kv) {
+    return mask && (mask_row < 0 || (B > 1 && mask_row < max_kv)) ? PQ_ERR_BAD_STRIDE : PQ_OK;
+}
+
+pq::PagedCache cache(const void* keys, const void* values, const uint8_t* codes, const void* rscale, const void* rmn, const void* tscale, const void* tmn,
+                     const int64_t* layout, const int32_t* q_start, const int32_t* kv_len, const int32_t* n_sealed, const int32_t* pages,
+                     const int32_t* value_pages, const int32_t* open_pages, int W, int Wo, int T, int B, int N, int Nk, int max_kv, int rbits, int tbits) {
+    pq::PagedCache c{};
+    c.keys = {keys, layout[0], layout[1], static_cast<int>(layout[8])};
+    c.values = {values, layout[2], layout[3], static_cast<int>(layout[9])};
+    c.codes = {codes, layout[4], layout[5], codes ? static_cast<int>(layout[10]) : 0};
+    c.meta = {nullptr, layout[6], layout[7], 0};
+    c.rscale = static_cast<const uint16_t*>(rscale);
+    c.rmn = static_cast<const uint16_t*>(rmn);
+    c.tscale = static_cast<const uint16_t*>(tscale);
+    c.tmn = static_cast<const uint16_t*>(tmn);
+    c.q_start = q_start;
+    c.kv_len = kv_len;
+    c.n_sealed = n_sealed;
+    c.pages = pages ? pages : value_pages;
+    c.value_pages = value_pages;
+    c.open_pages = open_pages;
+    c.W = W; c.Wo = Wo; c.T = T; c.B = B; c.N = N; c.Nk = Nk; c.max_kv = max_kv; c.rbits = rbits; c.tbits = tbits;
+    return c;
+}
+
+}  // namespace
+
+extern "C" {
+
+int pq_validate_paged_append(const void* q, int64_t q_row, const void* k, int64_t k_row, const void* v, int64_t v_row, const void* cos, const void* sin,
+                             int64_t angle_rows, const int32_t* positions, const void* q_norm, const void* k_norm, const void* q_out, const void* keys,
+                             const void* values, const int64_t* layout, const int32_t* q_start, const int32_t* kv_len, const int32_t* n_sealed,
+                             const int32_t* value_pages, const int32_t* open_pages, int W, int Wo, int T, int B, int N, int Nk, int max_q, int max_kv, int dtype) {
+    if (!cos || !sin || !q_out) return PQ_ERR_NULL_POINTER;
+    if (!half_dtype(dtype)) return PQ_ERR_BAD_DTYPE;
+    if (int rc = check_counts(q_start, kv_len, n_sealed, W, Wo, T, B, N, Nk, max_q, max_kv)) return rc;
+    if (int rc = check_layout(layout, keys, values, nullptr, nullptr, nullptr, nullptr, nullptr)) return rc;
+    if (int rc = check_pages(nullptr, nullptr, value_pages, open_pages, Wo, 4, 4, 0)) return rc;
+    if (angle_rows < 1) return PQ_ERR_BAD_SHAPE;
+    if (int rc = check_queries(q, q_row, N, T)) return rc;
+    if (int rc = check_queries(k, k_row, Nk, T)) return rc;
+    if (int rc = check_queries(v, v_row, Nk, T)) return rc;
+    if (!aligned(cos, 16) || !aligned(sin, 16) || !aligned(q_norm, 16) || !aligned(k_norm, 16) || !aligned(q_out, 16) || !aligned(positions, 4))
+        return PQ_ERR_MISALIGNED;
+    return PQ_OK;
+}
+
+int pq_paged_append(const void* q, int64_t q_row, const void* k, int64_t k_row, const void* v, int64_t v_row, const void* cos, const void* sin,
+                    int64_t angle_rows, const int32_t* positions, const void* q_norm, const void* k_norm, float eps, void* q_out, void* keys, void* values,
+                    const int64_t* layout, const int32_t* q_start, const int32_t* kv_len, const int32_t* n_sealed, const int32_t* value_pages,
+                    const int32_t* open_pages, int W, int Wo, int T, int B, int N, int Nk, int max_q, int max_kv, int dtype, void* stream) {
+    if (int rc = pq_validate_paged_append(q, q_row, k, k_row, v, v_row, cos, sin, angle_rows, positions, q_norm, k_norm, q_out, keys, values, layout, q_start,
+                                          kv_len, n_sealed, value_pages, open_pages, W, Wo, T, B, N, Nk, max_q, max_kv, dtype))
+        return rc;
+    pq::PagedAppendArgs a{};
+    a.c = cache(keys, values, nullptr, nullptr, nullptr, nullptr, nullptr, layout, q_start, kv_len, n_sealed, nullptr, value_pages, open_pages, W, Wo, T, B, N, Nk,
+                max_kv, 4, 4);
+    a.q = static_cast<const uint16_t*>(q); a.k = static_cast<const uint16_t*>(k); a.v = static_cast<const uint16_t*>(v);
+    a.q_row = q_row; a.k_row = k_row; a.v_row = v_row;
+    a.cos = static_cast<const uint16_t*>(cos); a.sin = static_cast<const uint16_t*>(sin);
+    a.angle_rows = angle_rows;
+    a.positions = positions;
+    a.q_norm = static_cast<const uint16_t*>(q_norm); a.k_norm = static_cast<const uint16_t*>(k_norm);
+    a.q_out = static_cast<uint16_t*>(q_out);
+    a.max_q = max_q;
+    a.eps = eps;
+    return status(pq::launch_paged_append(a, dtype, static_cast<hipStream_t>(stream)));
+}
+
+int pq_paged_attn_plan(int B, int N, int Nk, int max_q, int max_kv, int n_cus) {
+    if (B < 1 || N < 1 || Nk < 1 || N % Nk || max_q < 1 || max_kv < 1) return 1;
+    return pq::paged_splits(B, N, Nk, max_q, max_kv, n_cus);
+}
+
+size_t pq_paged_attn_workspace_bytes(int T, int N, int n_splits) {
+    if (T < 1 || N < 1 || n_splits <= 1) return 0;
+    return static_cast<size_t>(T) * N * n_splits * (PQ_HEAD_DIM + 2) * sizeof(float);
+}
+
+int pq_validate_paged_attn(const void* q, int64_t q_row, const void* keys, const void* values, const uint8_t* codes, const void* rscale, const void* rmn,
+                           const void* tscale, const void* tmn, const int64_t* layout, const int32_t* q_start, const int32_t* kv_len, const int32_t* n_sealed,
+                           const int32_t* pages, const int32_t* value_pages, const int32_t* open_pages, int W, int Wo, const uint8_t* mask, int64_t mask_row,
+                           const void* out, const float* lse, int T, int B, int N, int Nk, int max_q, int max_kv, int rbits, int tbits, int n_splits,
+                           const void* workspace, size_t workspace_bytes, int dtype, unsigned flags) {
+    if (!out) return PQ_ERR_NULL_POINTER;
+    if (!half_dtype(dtype)) return PQ_ERR_BAD_DTYPE;
+    if (int rc = check_counts(q_start, kv_len, n_sealed, W, Wo, T, B, N, Nk, max_q, max_kv)) return rc;
+    if (int rc = check_layout(layout, keys, values, codes, rscale, rmn, tscale, tmn)) return rc;
+    if (int rc = check_pages(codes, pages, value_pages, open_pages, Wo, rbits, tbits, flags)) return rc;
+    if (int rc = check_queries(q, q_row, N, T)) return rc;
+    if (int rc = check_mask(mask, mask_row, B, max_kv)) return rc;
+    const int64_t rows = static_cast<int64_t>(max_q) * (N / Nk), tile = pq::paged_tile_rows(rows);
+    if (n_splits < 1 || (rows + tile - 1) / tile * n_splits > 65535 || (static_cast<int64_t>(max_q) * N + 3) / 4 > INT32_MAX) return PQ_ERR_BAD_SHAPE;
+    if (!aligned(out, 16) || !aligned(lse, 4) || !aligned(workspace, 16)) return PQ_ERR_MISALIGNED;
+    if (n_splits > 1) {
+        if (!workspace) return PQ_ERR_NULL_POINTER;
+        if (workspace_bytes < pq_paged_attn_workspace_bytes(T, N, n_splits)) return PQ_ERR_WORKSPACE;
+    }
+    return PQ_OK;
+}
+
+int pq_paged_attn(const void* q, int64_t q_row, const void* keys, const void* values, const uint8_t* codes, const void* rscale, const void* rmn,
+                  const void* tscale, const void* tmn, const int64_t* layout, const int32_t* q_start, const int32_t* kv_len, const int32_t* n_sealed,
+                  const int32_t* pages, const int32_t* value_pages, const int32_t* open_pages, int W, int Wo, const uint8_t* mask, int64_t mask_row, void* out,
+                  float* lse, int T, int B, int N, int Nk, int max_q, int max_kv, int rbits, int tbits, float scale, int n_splits, int n_cus, void* workspace,
+                  size_t workspace_bytes, int dtype, unsigned flags, void* stream) {
+    if (int rc = pq_validate_paged_attn(q, q_row, keys, values, codes, rscale, rmn, tscale, tmn, layout, q_start, kv_len, n_sealed, pages, value_pages, open_pages,
+                                        W, Wo, mask, mask_row, out, lse, T, B, N, Nk, max_q, max_kv, rbits, tbits, n_splits, workspace, workspace_bytes, dtype, flags))
+        return rc;
+    pq::PagedAttnArgs a{};
+    a.c = cache(keys, values, codes, rscale, rmn, tscale, tmn, layout, q_start, kv_len, n_sealed, pages, value_pages, open_pages, W, Wo, T, B, N, Nk,
+                max_kv, rbits, tbits);
+    a.q = static_cast<const uint16_t*>(q);
+    a.q_row = q_row;
+    a.mask = mask;
+    a.mask_row = mask_row;
+    a.out = static_cast<uint16_t*>(out);
+    a.lse = lse;
+    a.partial = static_cast<float*>(workspace);
+    a.max_q = max_q;
+    a.n_splits = n_splits;
+    a.slots = 2 * (n_cus > 0 ? n_cus : 256);
+    a.scale = scale;
+    return status(pq::launch_paged_token(a, dtype, (flags & PQ_CODES_PACKED6) != 0, static_cast<hipStream_t>(stream)));
+}
+
+int pq_validate_paged_weights(const void* q, int64_t q_row, const float* lse, const void* keys, const uint8_t* codes, const void* rscale, const void* rmn,
+                              const void* tscale, const void* tmn, const int64_t* layout, const int32_t* q_start, const int32_t* kv_len,
+                              const int32_t* n_sealed, const int32_t* pages, const int32_t* value_pages, const int32_t* open_pages, int W, int Wo,
+                              const uint8_t* mask, int64_t mask_row, const float* onto, const float* weights, int T, int B, int N, int Nk, int max_q,
+                              int max_kv, int rbits, int tbits, int dtype, unsigned flags) {
+    if (!lse || !weights) return PQ_ERR_NULL_POINTER;
+    if (!half_dtype(dtype)) return PQ_ERR_BAD_DTYPE;
+    if (int rc = check_counts(q_start, kv_len, n_sealed, W, Wo, T, B, N, Nk, max_q, max_kv)) return rc;
+    if (int rc = check_layout(layout, keys, keys, codes, rscale, rmn, tscale, tmn)) return rc;
+    if (int rc = check_pages(codes, pages, value_pages, open_pages, Wo, rbits, tbits, flags)) return rc;
+    if (int rc = check_queries(q, q_row, N, T)) return rc;
+    if (int rc = check_mask(mask, mask_row, B, max_kv)) return rc;
+    if (W > 65535) return PQ_ERR_BAD_SHAPE;
+    return aligned(lse, 4) && aligned(weights, 4) && aligned(onto, 4) ? PQ_OK : PQ_ERR_MISALIGNED;
+}
+
+int pq_paged_weights(const void* q, int64_t q_row, const float* lse, const void* keys, const uint8_t* codes, const void* rscale, const void* rmn,
+                     const void* tscale, const void* tmn, const int64_t* layout, const int32_t* q_start, const int32_t* kv_len, const int32_t* n_sealed,
+                     const int32_t* pages, const int32_t* value_pages, const int32_t* open_pages, int W, int Wo, const uint8_t* mask, int64_t mask_row,
+                     const float* onto, float* weights, int T, int B, int N, int Nk, int max_q, int max_kv, int rbits, int tbits, float scale, int dtype,
+                     unsigned flags, void* stream) {
+    if (int rc = pq_validate_paged_weights(q, q_row, lse, keys, codes, rscale, rmn, tscale, tmn, layout, q_start, kv_len, n_sealed, pages, value_pages, open_pages, W,
+                                           Wo, mask, mask_row, onto, weights, T, B, N, Nk, max_q, max_kv, rbits, tbits, dtype, flags))
+        return rc;
+    pq::PagedWeightArgs a{};
+    a.c = cache(keys, nullptr, codes, rscale, rmn, tscale, tmn, layout, q_start, kv_len, n_sealed, pages, value_pages, open_pages, W, Wo, T, B, N, Nk,
+                max_kv, rbits, tbits);
+    a.q = static_cast<const uint16_t*>(q);
+    a.q_row = q_row;
+    a.mask = mask;
+    a.mask_row = mask_row;
+    a.lse = lse;
+    a.onto = onto;
+    a.weights = weights;
+    a.max_q = max_q;
+    a.scale = scale;
+    return status(pq::launch_paged_weights(a, dtype, (flags & PQ_CODES_PACKED6) != 0, static_cast<hipStream_t>(stream)));
+}
+
+int pq_validate_evict_pages(const float* weights, const int32_t* pages, const int32_t* n_sealed, const int32_t* kv_len, int B, int Nk, int W, int keep, int sinks,
+                            const int32_t* pages_out, const int32_t* n_sealed_out, const int32_t* kv_len_out, const float* weights_out, const int32_t* freed) {
+    if (!weights || !pages || !n_sealed || !kv_len || !pages_out || !n_sealed_out || !kv_len_out || !weights_out || !freed) return PQ_ERR_NULL_POINTER;
+    if (B < 1 || Nk < 1 || W < 1 || W > PQ_EVICT_MAX_PAGES || sinks < 0 || keep < 1 || keep < sinks) return PQ_ERR_BAD_SHAPE;
+    // (places are written while others are read)
+    if (pages_out == pages || weights_out == weights || freed == pages || freed == pages_out || n_sealed_out == n_sealed || kv_len_out == kv_len) return PQ_ERR_BAD_SHAPE;
+    return PQ_OK;
+}
+
+int pq_evict_pages(const float* weights, const int32_t* pages, const int32_t* n_sealed, const int32_t* kv_len, int B, int Nk, int W, int keep, int sinks,
+                   int32_t* pages_out, int32_t* n_sealed_out, int32_t* kv_len_out, float* weights_out, int32_t* freed, void* stream) {
+    if (int rc = pq_validate_evict_pages(weights, pages, n_sealed, kv_len, B, Nk, W, keep, sinks, pages_out, n_sealed_out, kv_len_out, weights_out, freed)) return rc;
+    pq::EvictArgs a{weights, pages, n_sealed, kv_len, pages_out, n_sealed_out, kv_len_out, freed, weights_out, B, Nk, W, keep, sinks};
+    return status(pq::launch_evict_pages(a, static_cast<hipStream_t>(stream)));
+}
+
+}  // extern "C"

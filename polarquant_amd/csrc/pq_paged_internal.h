@@ -1,0 +1,79 @@
+// Argument blocks and launcher prototypes of the paged cache's kernels (pq_paged_token.hip, pq_paged_chunk.hip, pq_paged_weights.hip, pq_paged_rows.hip),
+// shared with their C-ABI translation unit.  Each launcher returns a hipError_t cast to int (0 = ok).  dtype: 0 float16, 1 bfloat16.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace pq {
+
+constexpr int kPageTokens = 128;
+
+// [pages, Nk, 128, ..]: element (page, head, ..) at page * page_stride + head * head_stride + ..
+struct PageStream {
+    const void* at;
+    int64_t page, head;
+    int n;                                    // physical pages
+};
+
+struct PagedCache {
+    PageStream keys, values, codes, meta;     // meta: strides of the four tensors of constants; n unused
+    const uint16_t *rscale, *rmn, *tscale, *tmn;
+    const int32_t *q_start, *kv_len, *n_sealed;          // [B + 1], [B], [B] (null: none is sealed)
+    const int32_t *pages, *value_pages, *open_pages;     // [B, W], [B, W], [B, Wo]
+    int W, Wo, T, B, N, Nk, max_kv, rbits, tbits;
+};
+
+struct PagedAttnArgs {
+    PagedCache c;
+    const uint16_t* q;                        // row (t, head) at t * q_row + head * 128
+    int64_t q_row;
+    const uint8_t* mask;                      // [B, >= max_kv] rows mask_row apart, or null
+    int64_t mask_row;
+    uint16_t* out;                            // [T, N, 128]
+    float* lse;                               // [T, N] or null
+    float* partial;                           // [T * N, n_splits, 128], then [T * N, n_splits] pairs (maximum in log2 units, sum)
+    int max_q, n_splits, slots;               // slices a sequence is cut into at most; workgroups that the device holds
+    float scale;
+};
+int launch_paged_token(const PagedAttnArgs& a, int dtype, bool packed, hipStream_t st);
+int launch_paged_merge(const PagedAttnArgs& a, int dtype, int tile_rows, hipStream_t st);
+
+struct PagedWeightArgs {
+    PagedCache c;
+    const uint16_t* q;
+    int64_t q_row;
+    const uint8_t* mask;
+    int64_t mask_row;
+    const float* lse;                         // [T, N]
+    const float* onto;                        // [B, Nk, W] or null
+    float* weights;                           // [B, Nk, W]
+    int max_q;
+    float scale;
+};
+int launch_paged_weights(const PagedWeightArgs& a, int dtype, bool packed, hipStream_t st);
+
+struct PagedAppendArgs {
+    PagedCache c;                             // keys and values are written
+    const uint16_t *q, *k, *v;                // rows q_row, k_row, v_row apart
+    int64_t q_row, k_row, v_row;
+    const uint16_t *cos, *sin;                // [angle_rows, 128]
+    int64_t angle_rows;
+    const int32_t* positions;                 // [T] or null: the tokens' places in their sequences
+    const uint16_t *q_norm, *k_norm;          // [128] or null
+    uint16_t* q_out;                          // [T, N, 128]
+    int max_q;
+    float eps;
+};
+int launch_paged_append(const PagedAppendArgs& a, int dtype, hipStream_t st);
+
+struct EvictArgs {
+    const float* weights;                     // [B, Nk, W]
+    const int32_t *pages, *n_sealed, *kv_len;
+    int32_t *pages_out, *n_sealed_out, *kv_len_out, *freed;
+    float* weights_out;
+    int B, Nk, W, keep, sinks;
+};
+int launch_evict_pages(const EvictArgs& a, hipStream_t st);
+
+}  // namespace pq

@@ -1,0 +1,220 @@
+// Rows into the pages of a cache, and pages out of its tables.
+#include "pq_paged_device.h"
+
+namespace pq {
+
+// A token's projected rows: queries and keys normed over their 128 channels each and rotated by the token's position, keys and values into their
+// pages.  All in float32, rounded once.
+//
+// grid (4 tokens, 16 heads, sequences).  16 lanes a row, 8 channels each; the channel 64 apart is 8 lanes away, one rotation of the row's lanes.  A
+// wavefront's four rows of four steps are all requested before the first is used.  What bounds it: memory, 512 bytes a row.
+template <typename T>
+__global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
+    const PagedCache& c = a.c;
+    const int b = blockIdx.z, lane = threadIdx.x & 63, j = lane & 15;
+    const PagedSequence s = own_sequence(c, b);
+    const int t = uniform(static_cast<int>(blockIdx.x) * 4 + static_cast<int>(threadIdx.x >> 6));
+    if (t >= s.rows) return;
+    const int64_t token = s.first + t;
+    const int N = c.N, Nk = c.Nk, heads = N + 2 * Nk, at = s.past + t;
+    // where the key and the value go
+    int kp = -1, vp = -1;
+    if (at >= 0) {
+        const int p = at / kPageTokens;
+        if (p >= s.sealed) kp = key_page(c, s, b, p);
+        vp = value_page(c, b, p);
+    }
+    int64_t angle = a.positions ? uniform(a.positions[token]) : at;
+    angle = angle < 0 ? 0 : angle >= a.angle_rows ? a.angle_rows - 1 : angle;
+    uint4 x[4];
+    int row[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        row[i] = blockIdx.y * 16 + 4 * i + (lane >> 4);
+        const int r = row[i] < heads ? row[i] : 0;
+        const uint16_t* from = r < N ? a.q + token * a.q_row + r * 128 : r < N + Nk ? a.k + token * a.k_row + (r - N) * 128 : a.v + token * a.v_row + (r - N - Nk) * 128;
+        x[i] = *reinterpret_cast<const uint4*>(from + 8 * j);
+    }
+    const uint4 cw = *reinterpret_cast<const uint4*>(a.cos + angle * 128 + 8 * j), sw = *reinterpret_cast<const uint4*>(a.sin + angle * 128 + 8 * j);
+    const uint4 none = make_uint4(0, 0, 0, 0);
+    const uint4 qw = a.q_norm ? *reinterpret_cast<const uint4*>(a.q_norm + 8 * j) : none, kw = a.k_norm ? *reinterpret_cast<const uint4*>(a.k_norm + 8 * j) : none;
+    auto element = [](const uint4& w, int e) {
+        const uint32_t v = e < 2 ? w.x : e < 4 ? w.y : e < 6 ? w.z : w.w;
+        return lo2f<T>(static_cast<uint16_t>(e & 1 ? v >> 16 : v & 0xffffu));
+    };
+    const float sign = j < 8 ? -1.0f : 1.0f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int r = row[i];
+        const bool query = r < N, key = !query && r < N + Nk;
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) y[e] = element(x[i], e);
+        if (a.q_norm || a.k_norm) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) sum = __builtin_fmaf(y[e], y[e], sum);
+            sum += __uint_as_float(row_rotate<8>(__float_as_uint(sum)));
+            sum += __uint_as_float(row_rotate<4>(__float_as_uint(sum)));
+            sum += __uint_as_float(row_rotate<2>(__float_as_uint(sum)));
+            sum += __uint_as_float(row_rotate<1>(__float_as_uint(sum)));
+            const float inv = rsqrtf(__builtin_fmaf(sum, 1.0f / 128.0f, a.eps));
+            const bool normed = query ? a.q_norm != nullptr : a.k_norm != nullptr;
+#pragma unroll
+            for (int e = 0; e < 8; e++) y[e] = normed ? y[e] * inv * element(query ? qw : kw, e) : y[e];
+        }
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+            float z[2];
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const float other = __uint_as_float(row_rotate<8>(__float_as_uint(y[e + k])));
+                z[k] = __builtin_fmaf(y[e + k], element(cw, e + k), sign * other * element(sw, e + k));
+            }
+            w[e / 2] = pack_pair<T>(z[0], z[1]);
+        }
+        const uint4 turned = make_uint4(w[0], w[1], w[2], w[3]);
+        if (query) {
+            *reinterpret_cast<uint4*>(a.q_out + (token * N + r) * 128 + 8 * j) = turned;
+        } else if (key) {
+            if (kp >= 0)
+                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(const_cast<void*>(c.keys.at)) + kp * c.keys.page + (r - N) * c.keys.head +
+                                          (at % kPageTokens) * 128 + 8 * j) = turned;
+        } else if (r < heads && vp >= 0) {
+            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(const_cast<void*>(c.values.at)) + vp * c.values.page + (r - N - Nk) * c.values.head +
+                                      (at % kPageTokens) * 128 + 8 * j) = x[i];
+        }
+    }
+}
+
+int launch_paged_append(const PagedAppendArgs& a, int dtype, hipStream_t st) {
+    const dim3 grid((a.max_q + 3) / 4, (a.c.N + 2 * a.c.Nk + 15) / 16, a.c.B), block(256);
+    if (dtype == 0) hipLaunchKernelGGL(paged_append_kernel<F16>, grid, block, 0, st, a);
+    else hipLaunchKernelGGL(paged_append_kernel<BF16>, grid, block, 0, st, a);
+    return static_cast<int>(hipGetLastError());
+}
+
+// Which sealed pages stay: the first `sinks`, and of the others those of the largest weight, the sum over the KV heads (in 64 bits, rounded to
+// 32), up to `keep` in all; of equal ones the earlier.  Tables and weights close up, in order.
+//
+// One workgroup a sequence.  The least weight that stays is found a byte at a time from the top, by counting (LDS atomics of integers, whose order
+// does not matter); places then are prefix sums over the pages in order.  What bounds it: the dozen barriers, some microseconds.
+constexpr int kEvictThreads = 1024;
+
+__global__ __launch_bounds__(kEvictThreads) void evict_pages_kernel(EvictArgs a) {
+    extern __shared__ uint32_t shared[];
+    uint32_t* rank = shared;                  // [W] a page's weight as an integer of the same order
+    int* from = reinterpret_cast<int*>(shared + a.W);                        // [W] logical page that comes to a place
+    __shared__ uint32_t count[256];
+    __shared__ uint32_t found[2];             // bits of the border so far; how many of them are still to be taken
+    __shared__ int waves[3][kEvictThreads / kWave];
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, W = a.W, b = blockIdx.x;
+    const int n = within(a.n_sealed[b], 0, W), keep = n < a.keep ? n : a.keep;
+    const int32_t* pages = a.pages + static_cast<int64_t>(b) * W;
+    const float* weights = a.weights + static_cast<int64_t>(b) * a.Nk * W;
+    for (int j = tid; j < n; j += kEvictThreads) {
+        double sum = 0.0;
+#pragma unroll 8
+        for (int h = 0; h < a.Nk; h++) sum += static_cast<double>(weights[static_cast<int64_t>(h) * W + j]);
+        const float f = static_cast<float>(sum) + 0.0f;                      // (minus zero is zero)
+        const uint32_t w = __float_as_uint(f);
+        rank[j] = j < a.sinks || f != f ? 0xffffffffu : w & 0x80000000u ? ~w : w | 0x80000000u;
+    }
+    if (tid == 0) { found[0] = 0; found[1] = keep; }
+    // the rank of the last page that stays (n > keep: otherwise all do)
+    if (n > keep) {
+        for (int shift = 24; shift >= 0; shift -= 8) {
+            if (tid < 256) count[tid] = 0;
+            __syncthreads();
+            const uint32_t prefix = found[0], above = shift == 24 ? 0u : ~0u << (shift + 8);
+            for (int j = tid; j < n; j += kEvictThreads) {
+                const uint32_t r = rank[j];
+                if ((r & above) == prefix) atomicAdd(&count[(r >> shift) & 255], 1u);
+            }
+            __syncthreads();
+            if (wv == 0) {                    // lane l: bytes 255 - 4 l .. 252 - 4 l, from the top
+                uint32_t own[4], sum = 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++) { own[i] = count[255 - 4 * lane - i]; sum += own[i]; }
+                uint32_t before = sum;
+#pragma unroll
+                for (int o = 1; o < 64; o <<= 1) {
+                    const uint32_t v = __shfl_up(before, o);
+                    before += lane >= o ? v : 0u;
+                }
+                before -= sum;
+                const uint32_t want = found[1];
+                if (before < want && want <= before + sum) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        if (before < want && want <= before + own[i]) {
+                            found[0] = prefix | static_cast<uint32_t>(255 - 4 * lane - i) << shift;
+                            found[1] = want - before;
+                        }
+                        before += own[i];
+                    }
+                }
+            }
+            __syncthreads();
+        }
+    }
+    __syncthreads();
+    const uint32_t border = found[0], ties = found[1];                       // of the pages at the border the first `ties` stay
+    // places, a thousand pages at a time
+    int tied = 0, left = 0, gone = 0;         // of the pages before
+    for (int j0 = 0; j0 < W; j0 += kEvictThreads) {
+        const int j = j0 + tid;
+        const int page = j < W ? pages[j] : -1;
+        const bool sealed = j < n, tie = sealed && n > keep && rank[j] == border;
+        const uint64_t tie_bits = __ballot(tie), before = (1ull << lane) - 1;
+        if (lane == 0) waves[0][wv] = __popcll(tie_bits);
+        __syncthreads();
+        int place = tied + __popcll(tie_bits & before);
+        for (int w = 0; w < kEvictThreads / kWave; w++) {
+            if (w < wv) place += waves[0][w];
+            tied += waves[0][w];
+        }
+        const bool stays = sealed ? n <= keep || rank[j] > border || (tie && static_cast<uint32_t>(place) < ties) : j < W && page >= 0;
+        const bool goes = sealed && !stays;
+        const uint64_t stay_bits = __ballot(stays), go_bits = __ballot(goes);
+        if (lane == 0) { waves[1][wv] = __popcll(stay_bits); waves[2][wv] = __popcll(go_bits); }
+        __syncthreads();
+        int to = left + __popcll(stay_bits & before), out = gone + __popcll(go_bits & before);
+        for (int w = 0; w < kEvictThreads / kWave; w++) {
+            if (w < wv) { to += waves[1][w]; out += waves[2][w]; }
+            left += waves[1][w];
+            gone += waves[2][w];
+        }
+        if (stays) { from[to] = j; a.pages_out[static_cast<int64_t>(b) * W + to] = page; }
+        if (goes) a.freed[static_cast<int64_t>(b) * W + out] = page;
+        __syncthreads();
+    }
+    for (int j = tid; j < W; j += kEvictThreads) {
+        if (j >= left) a.pages_out[static_cast<int64_t>(b) * W + j] = -1;
+        if (j >= gone) a.freed[static_cast<int64_t>(b) * W + j] = -1;
+        float* out = a.weights_out + static_cast<int64_t>(b) * a.Nk * W + j;
+        const int src = j < left ? from[j] : 0;
+#pragma unroll 4
+        for (int h = 0; h < a.Nk; h++) {
+            const float v = weights[static_cast<int64_t>(h) * W + src];
+            out[static_cast<int64_t>(h) * W] = j < left ? v : 0.0f;
+        }
+    }
+    if (tid == 0) {
+        a.n_sealed_out[b] = keep;
+        a.kv_len_out[b] = a.kv_len[b] - kPageTokens * (n - keep);
+    }
+}
+
+int launch_evict_pages(const EvictArgs& a, hipStream_t st) {
+    const size_t bytes = 8 * static_cast<size_t>(a.W);
+    if (bytes > 60 * 1024) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&evict_pages_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+        if (e != hipSuccess) return static_cast<int>(e);
+    }
+    hipLaunchKernelGGL(evict_pages_kernel, dim3(a.B), dim3(kEvictThreads), bytes, st, a);
+    return static_cast<int>(hipGetLastError());
+}
+
+}  // namespace pq

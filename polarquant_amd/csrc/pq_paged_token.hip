@@ -1,0 +1,446 @@
+// Attention over the pages of a cache, for few query rows a sequence (a row: a new token and a query head), and the merge of its slices.
+//
+// grid (KV heads, slices x row tiles, sequences).  A workgroup owns 16 NQ rows and a slice of whole pages; its four wavefronts divide the slice's
+// blocks of 32 tokens among them and run on their own until their states are joined in LDS, so nothing waits at a barrier.  As in the prompt
+// kernel the score tile is transposed, S^T = K Q^T: a row is a lane, its softmax state a register, and the weights are the right operand of
+// O^T = V^T P^T as they stand.  The left operand of S^T has a key's row in a lane, 16 pairs in each of the four lanes of a key: what a lane
+// loads of the codes (16 bytes) becomes its operand without passing through LDS.
+//
+// Angles go through a table of cos and sin in LDS, 64 pairs x 16 bins of float16, which a wavefront makes once a page: word (pair % 16) 64 +
+// (pair / 16) 16 + bin, so that the lanes of a lookup, four pairs and sixteen keys, meet a bank only with a lane that wants the same word.
+// (More than 16 bins: cos and sin are evaluated for every code.)  Radii are (code) x (width of a bin) + (least and half a width).
+#include "pq_paged_device.h"
+
+namespace pq {
+
+constexpr int kTokenBlock = 32, kTokenValues = kTokenBlock * 256, kTokenTable = 4096, kTokenWave = 2 * kTokenValues + kTokenTable;
+
+template <typename T, int NQ, bool PK6, bool TABLE>
+__global__ __launch_bounds__(256, 2) void paged_token_kernel(PagedAttnArgs a) {
+    extern __shared__ __attribute__((aligned(1024))) uint8_t sm[];
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, g = lane >> 4;
+    const int b = blockIdx.z, h = blockIdx.x, slice = blockIdx.y % a.n_splits, tile = blockIdx.y / a.n_splits;
+    const PagedCache& c = a.c;
+    const PagedSequence s = own_sequence(c, b);
+    const int rep = c.N / c.Nk, rows = s.rows * rep, row0 = tile * 16 * NQ;
+    if (row0 >= rows) return;
+    const int pages = (s.kv + kPageTokens - 1) / kPageTokens;
+    const int per = pages_per_slice(c, pages, a.n_splits, a.slots, 16 * NQ);
+    if (slice > 0 && slice * per >= pages) return;
+    const bool only = per >= pages;
+
+    const uint32_t lds0 = uniform(lds_addr(sm) + wv * kTokenWave), table = lds0 + 2 * kTokenValues;
+
+    // this lane's rows, the keys they see, and their queries: 16 channels from 16 g on and 16 from 64 + 16 g on, which is the order of a key's pairs
+    const float scale2 = a.scale != 0.0f ? fabsf(a.scale) * kLog2e : 1.0f;
+    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u, keep = a.scale != 0.0f ? 0xffffffffu : 0u;
+    int limit[NQ];
+    const uint16_t* qp[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+        const int r = row0 + 16 * n + r16, rc = r < rows ? r : rows - 1, t = rc / rep;
+        limit[n] = r < rows ? s.past + t : -1;
+        qp[n] = a.q + (s.first + t) * a.q_row + (h * rep + rc % rep) * 128 + 16 * g;
+    }
+    u32x4_a q[NQ][4];
+    auto load_queries = [&]() {
+#pragma unroll
+        for (int n = 0; n < NQ; n++) {
+            u32x4_a w[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) w[i] = *reinterpret_cast<const u32x4_a*>(qp[n] + (i >> 1) * 64 + (i & 1) * 8);
+#pragma unroll
+            for (int i = 0; i < 4; i++) w[i] = u32x4_a{(w[i].x ^ flip) & keep, (w[i].y ^ flip) & keep, (w[i].z ^ flip) & keep, (w[i].w ^ flip) & keep};
+            q[n][0] = u32x4_a{w[0].x, w[0].y, w[2].x, w[2].y};
+            q[n][1] = u32x4_a{w[0].z, w[0].w, w[2].z, w[2].w};
+            q[n][2] = u32x4_a{w[1].x, w[1].y, w[3].x, w[3].y};
+            q[n][3] = u32x4_a{w[1].z, w[1].w, w[3].z, w[3].w};
+        }
+    };
+    const int first_limit = s.past + row0 / rep;                             // of the tile's rows: the least, the largest
+    const int last_row = row0 + 16 * NQ - 1 < rows - 1 ? row0 + 16 * NQ - 1 : rows - 1, last_limit = s.past + last_row / rep;
+
+    // this wavefront's blocks
+    int blocks = (s.kv + kTokenBlock - 1) / kTokenBlock;
+    const int p0 = slice * per, p1 = p0 + per < pages ? p0 + per : pages;
+    const int mine = (4 * (p1 - p0) + 3) / 4;
+    int blk0 = 4 * p0 + wv * mine, blk1 = blk0 + mine;
+    if (blk1 > 4 * p1) blk1 = 4 * p1;
+    const int seen = last_limit < 0 ? 0 : last_limit / kTokenBlock + 1;
+    if (blocks > seen) blocks = seen;
+    if (blk1 > blocks) blk1 = blocks;
+    const int border = 4 * s.sealed;
+
+    floatx4_a o[NQ][8];
+    float m[NQ], l[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+        m[n] = kNone;
+        l[n] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) o[n][i] = floatx4_a{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    // where 16 lanes read 4 tokens x 16 channels of the values and get them transposed, and what lane's 16 bytes go there: pieces of 16 bytes are
+    // swizzled by the token so that 8 tokens' reads of 32 bytes meet every bank once
+    uint32_t tops[8];                                                        // of channel tile i: chunks 2 i and 2 i + 1
+    {
+        const int row = 4 * g + (r16 >> 2);
+#pragma unroll
+        for (int i = 0; i < 8; i++) tops[i] = lds0 + row * 256 + ((2 * i + ((lane & 3) >> 1)) ^ ((row & 7) << 1)) * 16 + (lane & 1) * 8;
+    }
+
+    const float rest = 1.0f / static_cast<float>(1 << c.tbits);
+    const uint32_t angles4 = ((1u << c.tbits) - 1u) * 0x01010101u;
+
+    auto walk = [&](auto SEALED, int blk, const int end) {
+        constexpr bool sealed = decltype(SEALED)::value;
+        using TQ = std::conditional_t<sealed, F16, T>;
+        if (blk >= end) return;
+        load_queries();
+        float sc[NQ], page_scale = 1.0f;
+#pragma unroll
+        for (int n = 0; n < NQ; n++) {
+            sc[n] = scale2;
+            if constexpr (sealed && std::is_same<T, BF16>::value) {
+                float most = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const uint32_t w = q[n][i][j];
+                        most = fmaxf(most, fmaxf(fabsf(lo2f<T>(static_cast<uint16_t>(w & 0xffffu))), fabsf(lo2f<T>(static_cast<uint16_t>(w >> 16)))));
+                    }
+                most = both_halves_max(both_rows_max(most));
+                const int e = exponent_above(most);
+                const float factor = __builtin_ldexpf(1.0f, within(kHalfTop - e, -120, 120));
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) q[n][i][j] = scaled_half<T>(q[n][i][j], factor);
+                sc[n] = scale2 * __builtin_ldexpf(1.0f, -within(kHalfTop - e, -120, 120));
+            }
+        }
+        constexpr int KR = sealed ? 2 : 8;
+        u32x4_a kr[KR], kn[KR];                                              // this block's keys, the next one's
+        uint32_t bits = 0, bits_next = 0;
+        // constants of a page: raw, as radii of this lane's 16 pairs, of which page
+        u32x4_a raw_rs[2], raw_rm[2];
+        uint16_t raw_ts = 0, raw_tm = 0;
+        float rs[16], of[16];
+        int page_in = -1, page_asked = -1;
+        auto issue = [&](int at, int buf) {
+            const int p = at >> 2, sub = at & 3;
+            const int kp = key_page(c, s, b, p), vp = value_page(c, b, p);
+            const int n = s.kv - at * kTokenBlock;
+            uint32_t seen = n >= 32 ? 0xffffffffu : (1u << n) - 1u;
+            if (a.mask) {
+                const int key = at * kTokenBlock + (lane & 31);
+                const bool on = key < s.kv && a.mask[b * a.mask_row + key] != 0;
+                seen &= static_cast<uint32_t>(__ballot(on));
+            }
+            if (kp < 0 || vp < 0) seen = 0;
+            bits_next = __builtin_amdgcn_readfirstlane(seen);
+            if (!bits_next) return;
+            const u32x4_a vb = rows_at(static_cast<const uint16_t*>(c.values.at) + vp * c.values.page + h * c.values.head + sub * (kTokenBlock * 128));
+            const int some = __builtin_ctz(bits_next);                       // rows that are not there are copies of one that is, with weight zero
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int row = 4 * i + (lane >> 4), chunk = r16 ^ ((row & 7) << 1), from = (bits_next >> row) & 1 ? row : some;
+                rows_to_lds(vb, from * 256 + chunk * 16, lds0 + buf * kTokenValues + i * 1024);
+            }
+            if constexpr (sealed) {
+                const uint8_t* cb = static_cast<const uint8_t*>(c.codes.at) + kp * c.codes.page + h * c.codes.head;
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const int row = sub * kTokenBlock + 16 * u + r16;
+                    if constexpr (PK6) {
+                        const uint32_t* w = reinterpret_cast<const uint32_t*>(cb + row * 48 + 12 * g);
+                        kn[u] = u32x4_a{w[0], w[1], w[2], 0u};
+                    } else {
+                        kn[u] = *reinterpret_cast<const u32x4_a*>(cb + row * 64 + 16 * g);
+                    }
+                }
+                if (p != page_asked) {
+                    const int64_t at_meta = kp * c.meta.page + h * c.meta.head;
+                    const u32x4_a* prs = reinterpret_cast<const u32x4_a*>(c.rscale + at_meta + 16 * g);
+                    const u32x4_a* prm = reinterpret_cast<const u32x4_a*>(c.rmn + at_meta + 16 * g);
+                    raw_rs[0] = prs[0]; raw_rs[1] = prs[1];
+                    raw_rm[0] = prm[0]; raw_rm[1] = prm[1];
+                    raw_ts = c.tscale[at_meta + lane];
+                    raw_tm = c.tmn[at_meta + lane];
+                    page_asked = p;
+                }
+            } else {
+                const uint16_t* kb = static_cast<const uint16_t*>(c.keys.at) + kp * c.keys.page + h * c.keys.head + sub * (kTokenBlock * 128);
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        kn[4 * u + i] = *reinterpret_cast<const u32x4_a*>(kb + (16 * u + r16) * 128 + 16 * g + (i >> 1) * 64 + (i & 1) * 8);
+            }
+        };
+        auto take_page = [&]() {
+            float most = 0.0f;
+            const float top = static_cast<float>(1 << c.rbits);
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const uint32_t ws = raw_rs[i >> 3][(i & 7) >> 1], wm = raw_rm[i >> 3][(i & 7) >> 1];
+                rs[i] = lo2f<T>(static_cast<uint16_t>(i & 1 ? ws >> 16 : ws & 0xffffu));
+                of[i] = lo2f<T>(static_cast<uint16_t>(i & 1 ? wm >> 16 : wm & 0xffffu));
+                most = fmaxf(most, __builtin_fmaf(fabsf(rs[i]), top, fabsf(of[i])));
+                of[i] = __builtin_fmaf(rs[i], 0.5f, of[i]);
+            }
+            most = both_halves_max(both_rows_max(most));
+            const int e = within(kHalfTop - exponent_above(most), -120, 120);
+            const float factor = __builtin_ldexpf(1.0f, e);
+            page_scale = __builtin_ldexpf(1.0f, -e);
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                rs[i] *= factor * rest;                                      // (a radius code comes as a byte, above the angle's bits)
+                of[i] *= factor;
+            }
+            const float ts = lo2f<T>(raw_ts) * kTurn, tm = __builtin_fmaf(ts, 0.5f, lo2f<T>(raw_tm) * kTurn);
+            if constexpr (TABLE) {
+                const uint32_t at = table + ((lane & 15) * 64 + g * 16) * 4;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    u32x4_a w;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) w[j] = cos_sin_half(__builtin_fmaf(static_cast<float>(4 * i + j), ts, tm));
+                    *lds_ptr<lds_u32x4>(at + 16 * i) = w;
+                }
+            } else {
+                *lds_ptr<lds_f2>(table + lane * 8) = floatx2_a{ts, tm};
+            }
+        };
+        auto key_piece = [&](uint32_t w, auto S) {
+            constexpr int st = decltype(S)::value;
+            float r[4];
+            uint32_t cs[4];
+            uint32_t r4 = w & ~angles4;
+            if constexpr (TABLE) {
+                uint32_t a4 = (w & angles4) << 2;
+                asm volatile("" : "+v"(a4), "+v"(r4));
+#pragma unroll
+                for (int k = 0; k < 4; k++) cs[k] = *lds_ptr<lds_u32>(table + g * 64 + ((a4 >> (8 * k)) & 0xffu) + (st * 4 + k) * 256);
+            } else {
+                const uint32_t a4 = w & angles4;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const floatx2_a t = *lds_ptr<lds_f2>(table + (16 * g + 4 * st + k) * 8);
+                    cs[k] = cos_sin_half(__builtin_fmaf(static_cast<float>((a4 >> (8 * k)) & 0xffu), t.x, t.y));
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) r[k] = __builtin_fmaf(static_cast<float>((r4 >> (8 * k)) & 0xffu), rs[4 * st + k], of[4 * st + k]);
+            return quad_of_pairs(r, cs);
+        };
+        auto compute = [&](int at, int buf) {
+            floatx4_a z[2][NQ];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+#pragma unroll
+                for (int n = 0; n < NQ; n++) z[u][n] = floatx4_a{0.0f, 0.0f, 0.0f, 0.0f};
+                static_for<4>([&](auto S) {
+                    constexpr int st = decltype(S)::value;
+                    u32x4_a kf;
+                    if constexpr (sealed) {
+                        uint32_t w;
+                        if constexpr (PK6) {
+                            const uint32_t d0 = kr[u].x, d1 = kr[u].y, d2 = kr[u].z;
+                            w = unpack_codes6(st == 0 ? d0 : st == 1 ? (d0 >> 24) | (d1 << 8) : st == 2 ? (d1 >> 16) | (d2 << 16) : d2 >> 8);
+                        } else {
+                            w = kr[u][st];
+                        }
+                        kf = key_piece(w, S);
+                    } else {
+                        const u32x4_a x = kr[4 * u + (st >> 1)], y = kr[4 * u + 2 + (st >> 1)];
+                        kf = st & 1 ? u32x4_a{x.z, x.w, y.z, y.w} : u32x4_a{x.x, x.y, y.x, y.y};
+                    }
+#pragma unroll
+                    for (int n = 0; n < NQ; n++) z[u][n] = mma16<TQ>(kf, q[n][st], z[u][n]);
+                });
+            }
+            const bool whole = bits == 0xffffffffu && at * kTokenBlock + kTokenBlock - 1 <= first_limit;
+            u32x4_a p[NQ];
+#pragma unroll
+            for (int n = 0; n < NQ; n++) {
+                const float f = sealed ? sc[n] * page_scale : sc[n];
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[e] = z[e >> 2][n][e & 3];
+                if (!whole) {
+                    const int last = limit[n] - at * kTokenBlock - 4 * g;
+                    const uint32_t there = bits >> (4 * g);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const int k = 16 * (e >> 2) + (e & 3);
+                        x[e] = k <= last && (there >> k & 1) ? x[e] : -INFINITY;
+                    }
+                }
+                float mx = x[0];
+#pragma unroll
+                for (int e = 1; e < 8; e++) mx = fmaxf(mx, x[e]);
+                mx = both_halves_max(both_rows_max(mx)) * f;
+                if (__any(mx > m[n])) {
+                    const float mn = fmaxf(m[n], mx), al = exp2_hw(m[n] - mn);
+                    l[n] *= al;
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) o[n][i][j] *= al;
+                    m[n] = mn;
+                }
+                float w[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    w[e] = exp2_hw(__builtin_fmaf(x[e], f, -m[n]));
+                    l[n] += w[e];
+                }
+                p[n] = u32x4_a{pack_pair<T>(w[0], w[1]), pack_pair<T>(w[2], w[3]), pack_pair<T>(w[4], w[5]), pack_pair<T>(w[6], w[7])};
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const u32x2_a w0 = __builtin_bit_cast(u32x2_a, __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_ptr<lds_short4>(tops[i] + buf * kTokenValues)));
+                const u32x2_a w1 = __builtin_bit_cast(u32x2_a, __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_ptr<lds_short4>(tops[i] + buf * kTokenValues + 16 * 256)));
+                const u32x4_a vf = {w0.x, w0.y, w1.x, w1.y};
+#pragma unroll
+                for (int n = 0; n < NQ; n++) o[n][i] = mma16<T>(vf, p[n], o[n][i]);
+            }
+        };
+        auto arrived = [&]() {
+            rows_arrived();
+            bits = bits_next;
+#pragma unroll
+            for (int i = 0; i < KR; i++) kr[i] = kn[i];
+        };
+        issue(blk, 0);
+        arrived();
+        for (int buf = 0; blk < end; blk++, buf ^= 1) {
+            if constexpr (sealed) {                                          // (before the next page's constants are asked for)
+                if (bits && page_in != (blk >> 2)) { take_page(); page_in = blk >> 2; }
+            }
+            if (blk + 1 < end) issue(blk + 1, buf ^ 1);
+            if (bits) compute(blk, buf);
+            arrived();
+        }
+    };
+    walk(std::true_type{}, blk0, blk1 < border ? blk1 : border);
+    walk(std::false_type{}, blk0 > border ? blk0 : border, blk1);
+
+    // the four wavefronts' states, joined in the place of their values
+    const uint32_t pairs = lds0 + 2 * kTokenValues;
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+        l[n] += __shfl_xor(l[n], 16);
+        l[n] += __shfl_xor(l[n], 32);
+        const int row = 16 * n + r16;
+        if (g == 0) *lds_ptr<lds_f2>(pairs + row * 8) = floatx2_a{m[n], l[n]};
+#pragma unroll
+        for (int i = 0; i < 8; i++) *lds_ptr<lds_f4>(lds0 + row * 512 + (((4 * i + g) ^ (row & 15)) * 16)) = float4_v{o[n][i][0], o[n][i][1], o[n][i][2], o[n][i][3]};
+    }
+    __syncthreads();
+    const uint32_t base = lds_addr(sm);
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+        const int row = 16 * n + (tid >> 4), r = row0 + row, ch = tid & 15;              // 16-byte pieces 2 ch and 2 ch + 1 of the row
+        float mw[4], lw[4], mx = kNone, sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            const floatx2_a v = *lds_ptr<lds_f2>(base + w * kTokenWave + 2 * kTokenValues + row * 8);
+            mw[w] = v.x; lw[w] = v.y;
+            mx = fmaxf(mx, v.x);
+        }
+        float acc[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            const float f = exp2_hw(mw[w] - mx);
+            sum = __builtin_fmaf(lw[w], f, sum);
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const float4_v v = *lds_ptr<lds_f4>(base + w * kTokenWave + row * 512 + ((2 * ch + k) ^ (row & 15)) * 16);
+                acc[4 * k] = __builtin_fmaf(v.x, f, acc[4 * k]); acc[4 * k + 1] = __builtin_fmaf(v.y, f, acc[4 * k + 1]);
+                acc[4 * k + 2] = __builtin_fmaf(v.z, f, acc[4 * k + 2]); acc[4 * k + 3] = __builtin_fmaf(v.w, f, acc[4 * k + 3]);
+            }
+        }
+        if (r >= rows) continue;
+        const size_t at = static_cast<size_t>(s.first + r / rep) * c.N + h * rep + r % rep;
+        if (only) {
+            const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+            *reinterpret_cast<uint4*>(a.out + at * 128 + 8 * ch) = make_uint4(pack_pair<T>(acc[0] * inv, acc[1] * inv), pack_pair<T>(acc[2] * inv, acc[3] * inv),
+                                                                              pack_pair<T>(acc[4] * inv, acc[5] * inv), pack_pair<T>(acc[6] * inv, acc[7] * inv));
+            if (a.lse && ch == 0) a.lse[at] = sum > 0.0f ? (mx + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f : -INFINITY;
+        } else {
+            float* to = a.partial + (at * a.n_splits + slice) * 128 + 8 * ch;
+            *reinterpret_cast<float4*>(to) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+            *reinterpret_cast<float4*>(to + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
+            if (ch == 0) *reinterpret_cast<float2*>(a.partial + static_cast<size_t>(c.T) * c.N * a.n_splits * 128 + 2 * (at * a.n_splits + slice)) = make_float2(mx, sum);
+        }
+    }
+}
+
+// One wavefront joins a row's slices: lane i the weight of slices i, i + 64, .., then two channels.
+template <typename T>
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a, int tile_rows) {
+    const PagedCache& c = a.c;
+    const int b = blockIdx.y, lane = threadIdx.x & 63;
+    const PagedSequence s = own_sequence(c, b);
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    if (i >= static_cast<int64_t>(s.rows) * c.N) return;
+    const int pages = (s.kv + kPageTokens - 1) / kPageTokens;
+    const int per = pages_per_slice(c, pages, a.n_splits, a.slots, tile_rows);
+    if (per >= pages) return;                                                // (written by its only slice)
+    const int n = (pages + per - 1) / per;
+    const size_t at = static_cast<size_t>(s.first) * c.N + i;
+    const float2* ml = reinterpret_cast<const float2*>(a.partial + static_cast<size_t>(c.T) * c.N * a.n_splits * 128) + at * a.n_splits;
+    float mx = kNone;
+    for (int j = lane; j < n; j += kWave) mx = fmaxf(mx, ml[j].x);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+    const float* part = a.partial + at * a.n_splits * 128 + 2 * lane;
+    float sum = 0.0f, x = 0.0f, y = 0.0f;
+#pragma unroll 8
+    for (int j = 0; j < n; j++) {
+        const float2 v = ml[j], p = *reinterpret_cast<const float2*>(part + j * 128);
+        const float f = exp2_hw(v.x - mx);
+        sum = __builtin_fmaf(v.y, f, sum);
+        x = __builtin_fmaf(p.x, f, x);
+        y = __builtin_fmaf(p.y, f, y);
+    }
+    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    *reinterpret_cast<uint32_t*>(a.out + at * 128 + 2 * lane) = pack_pair<T>(x * inv, y * inv);
+    if (a.lse && lane == 0) a.lse[at] = sum > 0.0f ? (mx + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f : -INFINITY;
+}
+
+int launch_paged_merge(const PagedAttnArgs& a, int dtype, int tile_rows, hipStream_t st) {
+    const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(a.max_q) * a.c.N + 3) / 4), a.c.B), block(256);
+    if (dtype == 0) hipLaunchKernelGGL(paged_merge_kernel<F16>, grid, block, 0, st, a, tile_rows);
+    else hipLaunchKernelGGL(paged_merge_kernel<BF16>, grid, block, 0, st, a, tile_rows);
+    return static_cast<int>(hipGetLastError());
+}
+
+template <typename T, int NQ, bool PK6, bool TABLE>
+static int launch_token(const PagedAttnArgs& a, hipStream_t st) {
+    constexpr int bytes = 4 * kTokenWave;
+    const void* f = reinterpret_cast<const void*>(&paged_token_kernel<T, NQ, PK6, TABLE>);
+    if (const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, bytes); e != hipSuccess) return static_cast<int>(e);
+    const int tiles = (a.max_q * (a.c.N / a.c.Nk) + 16 * NQ - 1) / (16 * NQ);
+    hipLaunchKernelGGL((paged_token_kernel<T, NQ, PK6, TABLE>), dim3(a.c.Nk, tiles * a.n_splits, a.c.B), dim3(256), bytes, st, a);
+    const int err = static_cast<int>(hipGetLastError());
+    return err || a.n_splits == 1 ? err : launch_paged_merge(a, std::is_same<T, F16>::value ? 0 : 1, 16 * NQ, st);
+}
+
+template <typename T, int NQ>
+static int launch_token_of(const PagedAttnArgs& a, bool packed, hipStream_t st) {
+    if (packed) return launch_token<T, NQ, true, true>(a, st);
+    return a.c.tbits <= 4 ? launch_token<T, NQ, false, true>(a, st) : launch_token<T, NQ, false, false>(a, st);
+}
+
+int launch_paged_token(const PagedAttnArgs& a, int dtype, bool packed, hipStream_t st) {
+    const bool few = a.max_q * (a.c.N / a.c.Nk) <= 16;
+    if (dtype == 0) return few ? launch_token_of<F16, 1>(a, packed, st) : launch_token_of<F16, 2>(a, packed, st);
+    return few ? launch_token_of<BF16, 1>(a, packed, st) : launch_token_of<BF16, 2>(a, packed, st);
+}
+
+}  // namespace pq

@@ -1,0 +1,174 @@
+// The attention weight that a call's queries give to each page of a cache: the sum over the page's tokens, the rows and a KV head's query heads of
+// exp(score - log sum), the log sums being the attention's.
+//
+// grid (KV heads, pages, sequences): a workgroup owns a page, so its sum is written once, without atomics, in one order.  Its four wavefronts hold 32
+// keys each in registers for as long as the rows stream past through LDS, 64 at a time, two buffers.  The transposed score tile, S^T = K Q^T, has a
+// row's log sum in a lane, and needs no maximum.
+//
+// The sums are float32 and are held to that: a sealed key is split in two 16-bit parts, whose products are both added (2^-22 of it left in float16, 2^-16
+// in bfloat16, at random over 128 keys and more).  cos and sin are evaluated once a code: a key's lane pair takes one half each.
+#include "pq_paged_device.h"
+
+namespace pq {
+
+constexpr int kWeightRows = 64, kWeightTile = kWeightRows * 256;
+
+template <typename T, bool PK6>
+__global__ __launch_bounds__(256, 2) void paged_weights_kernel(PagedWeightArgs a) {
+    __shared__ __attribute__((aligned(1024))) uint8_t sm[2 * kWeightTile];
+    __shared__ float sums[4];
+    const PagedCache& c = a.c;
+    const int tid = threadIdx.x, lane = tid & 63, wv = uniform(tid >> 6), col = lane & 31, hi = lane >> 5;
+    const int b = blockIdx.z, h = blockIdx.x, p = blockIdx.y;
+    const PagedSequence s = own_sequence(c, b);
+    const int64_t entry = (static_cast<int64_t>(b) * c.Nk + h) * c.W + p;
+    const float had = a.onto ? a.onto[entry] : 0.0f;
+    const int rep = c.N / c.Nk, rows = s.rows * rep, key0 = p * kPageTokens + 32 * wv;
+    const bool any = p * kPageTokens < s.kv;
+    const int kp = any ? key_page(c, s, b, p) : -1, vp = any ? uniform(c.value_pages[static_cast<int64_t>(b) * c.W + p]) : -1;
+    // the first row that sees the page
+    const int first = p * kPageTokens - s.past > 0 ? (p * kPageTokens - s.past) * rep : 0, tile0 = first / kWeightRows;
+    const int tiles = (rows + kWeightRows - 1) / kWeightRows;
+    if (!any || kp < 0 || vp < 0 || tile0 >= tiles) {
+        if (tid == 0) a.weights[entry] = had;
+        return;
+    }
+    const uint32_t lds0 = lds_addr(sm);
+    auto fetch = [&](int tile, int buf) {
+        const int t0 = tile * kWeightRows / rep;
+        const u32x4_a qb = rows_at(a.q + (s.first + t0) * a.q_row + h * rep * 128);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int row = (wv * 4 + i) * 4 + (lane >> 4), chunk = (lane & 15) ^ (row & 15);
+            int r = tile * kWeightRows + row;
+            r = r < rows ? r : rows - 1;
+            rows_to_lds(qb, static_cast<uint32_t>(r / rep - t0) * static_cast<uint32_t>(2 * a.q_row) + (r % rep) * 256 + chunk * 16, lds0 + buf * kWeightTile + (wv * 4 + i) * 1024);
+        }
+    };
+    fetch(tile0, 0);
+    // this wavefront's keys that exist
+    const int n = s.kv - key0;
+    uint32_t bits = n >= 32 ? 0xffffffffu : n > 0 ? (1u << n) - 1u : 0u;
+    if (a.mask) {
+        const int key = key0 + col;
+        bits &= static_cast<uint32_t>(__ballot(key < s.kv && a.mask[b * a.mask_row + key] != 0));
+    }
+    bits = uniform(bits);
+    // key `col`, channels 64 hi .. 64 hi + 63
+    const bool sealed = p < s.sealed;
+    u32x4_a kf[8], kl[8];
+    if (sealed) {
+        const uint8_t* row = static_cast<const uint8_t*>(c.codes.at) + kp * c.codes.page + h * c.codes.head + (32 * wv + col) * (PK6 ? 48 : 64);
+        const int64_t meta = kp * c.meta.page + h * c.meta.head;
+        const uint32_t angles = (1u << c.tbits) - 1u;
+        uint32_t words[16];
+        if constexpr (PK6) {
+            u32x4_a w[3];
+#pragma unroll
+            for (int i = 0; i < 3; i++) w[i] = *reinterpret_cast<const u32x4_a*>(row + 16 * i);
+            uint32_t d[12];
+#pragma unroll
+            for (int i = 0; i < 12; i++) d[i] = w[i >> 2][i & 3];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                words[4 * i] = unpack_codes6(d[3 * i]);
+                words[4 * i + 1] = unpack_codes6((d[3 * i] >> 24) | (d[3 * i + 1] << 8));
+                words[4 * i + 2] = unpack_codes6((d[3 * i + 1] >> 16) | (d[3 * i + 2] << 16));
+                words[4 * i + 3] = unpack_codes6(d[3 * i + 2] >> 8);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const u32x4_a w = *reinterpret_cast<const u32x4_a*>(row + 16 * i);
+#pragma unroll
+                for (int j = 0; j < 4; j++) words[4 * i + j] = w[j];
+            }
+        }
+        const float quarter = hi ? 0.0f : 0.25f;                             // (a cosine is the sine a quarter turn on)
+        static_for<16>([&](auto I) {
+            constexpr int i = decltype(I)::value;
+            const uint2 wr = *reinterpret_cast<const uint2*>(c.rscale + meta + 4 * i), wm = *reinterpret_cast<const uint2*>(c.rmn + meta + 4 * i);
+            const uint2 wt = *reinterpret_cast<const uint2*>(c.tscale + meta + 4 * i), wn = *reinterpret_cast<const uint2*>(c.tmn + meta + 4 * i);
+            float v[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                auto half = [&](const uint2& w) { return lo2f<T>(static_cast<uint16_t>((k < 2 ? w.x : w.y) >> (16 * (k & 1)))); };
+                const uint32_t code = (words[i] >> (8 * k)) & 0xffu;
+                const float r = __builtin_fmaf(static_cast<float>(code >> c.tbits) + 0.5f, half(wr), half(wm));
+                const float turns = __builtin_fmaf(static_cast<float>(code & angles) + 0.5f, half(wt), half(wn)) * kTurn + quarter;
+                v[k] = r * __builtin_amdgcn_sinf(turns);
+            }
+            const uint32_t a0 = pack_pair<T>(v[0], v[1]), a1 = pack_pair<T>(v[2], v[3]);
+            auto rest = [&](uint32_t w, float x, float y) {
+                return pack_pair<T>(x - lo2f<T>(static_cast<uint16_t>(w & 0xffffu)), y - lo2f<T>(static_cast<uint16_t>(w >> 16)));
+            };
+            kf[i >> 1][2 * (i & 1)] = a0;
+            kf[i >> 1][2 * (i & 1) + 1] = a1;
+            kl[i >> 1][2 * (i & 1)] = rest(a0, v[0], v[1]);
+            kl[i >> 1][2 * (i & 1) + 1] = rest(a1, v[2], v[3]);
+        });
+    } else {
+        const uint16_t* row = static_cast<const uint16_t*>(c.keys.at) + kp * c.keys.page + h * c.keys.head + (32 * wv + col) * 128 + 64 * hi;
+#pragma unroll
+        for (int i = 0; i < 8; i++) kf[i] = *reinterpret_cast<const u32x4_a*>(row + 8 * i);
+#pragma unroll
+        for (int i = 0; i < 8; i++) kl[i] = u32x4_a{0u, 0u, 0u, 0u};
+    }
+    const float scale2 = a.scale * kLog2e;
+    float total = 0.0f;
+    rows_arrived();
+    __syncthreads();
+    for (int tile = tile0; tile < tiles; tile++) {
+        const int buf = (tile - tile0) & 1;
+        if (tile + 1 < tiles) fetch(tile + 1, buf ^ 1);
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const int r = tile * kWeightRows + 32 * u + col, rc = r < rows ? r : rows - 1, t = rc / rep;
+            float sum2 = a.lse[static_cast<int64_t>(s.first + t) * c.N + h * rep + rc % rep] * kLog2e;
+            sum2 = r < rows && sum2 != -INFINITY ? sum2 : INFINITY;          // (no row there, or one that saw nothing: no weight)
+            floatx16_a z;
+#pragma unroll
+            for (int j = 0; j < 16; j++) z[j] = 0.0f;
+            u32x4_a q[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) q[i] = *lds_ptr<lds_u32x4>(lds0 + buf * kWeightTile + (32 * u + col) * 256 + ((8 * hi + i) ^ (col & 15)) * 16);
+#pragma unroll
+            for (int i = 0; i < 8; i++) z = mma32<T>(kf[i], q[i], z);
+            if (sealed) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) z = mma32<T>(kl[i], q[i], z);
+            }
+            const int first_limit = s.past + (tile * kWeightRows + 32 * u) / rep;
+            if (bits != 0xffffffffu || key0 + 31 > first_limit) {
+                const int last = s.past + t - key0 - 4 * hi;
+                const uint32_t there = bits >> (4 * hi);
+#pragma unroll
+                for (int j = 0; j < 16; j++) {
+                    const int e = 8 * (j >> 2) + (j & 3);
+                    const float w = exp2_hw(__builtin_fmaf(z[j], scale2, -sum2));
+                    total += e <= last && (there >> e & 1) ? w : 0.0f;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 16; j++) total += exp2_hw(__builtin_fmaf(z[j], scale2, -sum2));
+            }
+        }
+        rows_arrived();
+        __syncthreads();
+    }
+    total = wave_sum(total);
+    if (lane == 0) sums[wv] = total;
+    __syncthreads();
+    if (tid == 0) a.weights[entry] = had + ((sums[0] + sums[1]) + (sums[2] + sums[3]));
+}
+
+int launch_paged_weights(const PagedWeightArgs& a, int dtype, bool packed, hipStream_t st) {
+    const dim3 grid(a.c.Nk, a.c.W, a.c.B), block(256);
+#define PQ_PW(T, P) hipLaunchKernelGGL((paged_weights_kernel<T, P>), grid, block, 0, st, a)
+    if (dtype == 0) { if (packed) PQ_PW(F16, true); else PQ_PW(F16, false); }
+    else            { if (packed) PQ_PW(BF16, true); else PQ_PW(BF16, false); }
+#undef PQ_PW
+    return static_cast<int>(hipGetLastError());
+}
+
+}  // namespace pq

@@ -39,29 +39,11 @@ __device__ __forceinline__ void load_to_lds(const void* p, uint32_t lds) {
 #pragma clang diagnostic pop
 __device__ __forceinline__ void wait_lds_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
-// the larger of lanes l and l ^ 32, by an exchange of half wavefronts that stays in the vector unit
-__device__ __forceinline__ float both_halves_max(float v) {
-    typedef unsigned int uint2_x __attribute__((ext_vector_type(2)));
-    const uint2_x r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(r.x), __uint_as_float(r.y));
-}
-
 // The order of a basic block's instructions by kind (a rule for the compiler's scheduler, which takes the calls in their order): so many
 // of one kind next.
 constexpr int kMatrix = 0x8, kDsRead = 0x100;
 template <int KIND, int N>
 __device__ __forceinline__ void order() { __builtin_amdgcn_sched_group_barrier(KIND, N, 0); }
-
-typedef float floatx2_a __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x2_a __attribute__((ext_vector_type(2)));
-typedef _Float16 halfx2_a __attribute__((ext_vector_type(2)));
-template <typename T> __device__ __forceinline__ uint32_t pack_pair(float a, float b);
-template <> __device__ __forceinline__ uint32_t pack_pair<BF16>(float a, float b) {
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector(floatx2_a{a, b}, bf16x2_a));
-}
-template <> __device__ __forceinline__ uint32_t pack_pair<F16>(float a, float b) {
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector(floatx2_a{a, b}, halfx2_a));
-}
 
 // grid (heads, query tiles, sequences), longest query tiles first.  Four wavefronts with 32 query rows each over 64-key tiles of K
 // and V that are double-buffered in LDS.  The transposed score tile S^T = K Q^T makes a query a lane, its softmax state a

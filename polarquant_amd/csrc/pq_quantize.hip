@@ -307,11 +307,12 @@ __device__ __forceinline__ uint32_t pack_angle_radius(float a, float r, float y,
     return ESTIMATE ? w : w & 0x7fff7fffu;
 }
 
-template <typename T, bool UNIFORM, bool PK6, bool LIBM>
+// PAGED: group blockIdx.x is that many pages behind its sequence's sealed ones, and quantized if the sequence fills it.
+template <typename T, bool UNIFORM, bool PK6, bool LIBM, bool PAGED = false>
 __global__ __launch_bounds__(kQThreads) void quantize_kernel(
     const uint16_t* __restrict__ k, int64_t sb, int64_t sh, int64_t st, int Nk, int rbits, int tbits, AngleMode am,
     uint8_t* __restrict__ codes, uint16_t* __restrict__ rscale, uint16_t* __restrict__ rmn,
-    uint16_t* __restrict__ tscale, uint16_t* __restrict__ tmn, int cap, int off) {
+    uint16_t* __restrict__ tscale, uint16_t* __restrict__ tmn, int cap, int off, SealPages pages) {
     // angle/radius words of the tile, entry-major so that a wavefront's accesses are contiguous
     __shared__ uint32_t pr[kEntries][kQThreads];
     __shared__ uint32_t red[2][4][kPairs];      // max / min, wavefront, pair
@@ -322,6 +323,15 @@ __global__ __launch_bounds__(kQThreads) void quantize_kernel(
     const int grp = blockIdx.x, bh = blockIdx.y;
     const int b = bh / Nk, h = bh - b * Nk;
     const uint16_t* kb = k + b * sb + h * sh + static_cast<int64_t>(grp) * kGroup * st;
+    int to_page = 0;
+    if constexpr (PAGED) {
+        const int sealed = pages.n_sealed ? pages.n_sealed[b] : 0, at = sealed + grp;
+        if (sealed < 0 || at >= pages.W || at >= pages.kv_len[b] / kGroup) return;
+        const int from = pages.open_pages[static_cast<int64_t>(b) * pages.Wo + grp];
+        to_page = pages.pages[static_cast<int64_t>(b) * pages.W + at];
+        if (static_cast<unsigned>(from) >= static_cast<unsigned>(pages.n_open) || static_cast<unsigned>(to_page) >= static_cast<unsigned>(pages.n_pages)) return;
+        kb = k + from * pages.key_page + h * pages.key_head;
+    }
 
     // ---- pass 1: cheap estimates for every entry; remember which entries need the exact routines
     // (all of a thread's keys are requested at once: two rows at a time, as the compiler has it, do not cover the way to memory)
@@ -416,7 +426,7 @@ __global__ __launch_bounds__(kQThreads) void quantize_kernel(
             return make_uint2(static_cast<uint32_t>(f2lo<T>(v[0])) | (static_cast<uint32_t>(f2lo<T>(v[1])) << 16),
                               static_cast<uint32_t>(f2lo<T>(v[2])) | (static_cast<uint32_t>(f2lo<T>(v[3])) << 16));
         };
-        const size_t mi = plane * kPairs + 4 * pq4;
+        const size_t mi = (PAGED ? to_page * pages.meta_page + h * pages.meta_head : plane * kPairs) + 4 * pq4;
         *reinterpret_cast<uint2*>(tscale + mi) = pack4(ts);
         *reinterpret_cast<uint2*>(tmn + mi) = pack4(tm);
         *reinterpret_cast<uint2*>(rscale + mi) = pack4(rs);
@@ -429,7 +439,7 @@ __global__ __launch_bounds__(kQThreads) void quantize_kernel(
         ttop[i] = clamp_bound(ts[i], (1 << tbits) - 1);
         rtop[i] = clamp_bound(rs[i], (1 << rbits) - 1);
     }
-    uint8_t* cb = codes + plane * (kGroup * (PK6 ? kPackedRowBytes : kPairs));
+    uint8_t* cb = codes + (PAGED ? to_page * pages.code_page + h * pages.code_head : plane * (kGroup * (PK6 ? kPackedRowBytes : kPairs)));
     // scales of 0 (degenerate pairs), infinities and the far ends of the bfloat16 range take the division
     bool fast = true;
     Inverse tinv[4], rinv[4];
@@ -574,14 +584,10 @@ int launch_selftest(int dtype, unsigned long long* counters, hipStream_t st) {
     return static_cast<int>(hipGetLastError());
 }
 
-int launch_quantize(const void* k, const int64_t* strides, int dtype, int B, int Nk, int Nb, int rbits, int tbits,
-                    unsigned flags, uint8_t* codes, void* rscale, void* rmn, void* tscale, void* tmn,
-                    int cap, int off, hipStream_t st) {
-    dim3 grid(Nb, B * Nk), block(kQThreads);
+static AngleMode angle_mode(int dtype, int tbits, unsigned flags) {
     const float two_pi_f = 6.28318548202514648438f;   // (float)(2*pi)
     // eager torch-CPU casts the python scalar 2*pi to the tensor dtype first: 6.28125 in both dtypes
     AngleMode am;
-    const bool uniform = (flags & 2u) != 0;
     am.two_pi = (flags & 1u) ? two_pi_f : 6.28125f;
     am.ttop = (1u << tbits) - 1u;
     am.minus_one = -1.0f;
@@ -591,12 +597,21 @@ int launch_quantize(const void* k, const int64_t* strides, int dtype, int B, int
     };
     am.tmn = round_dt(-3.14159274101257324219f);
     am.tscale = round_dt(round_dt(two_pi_f) / static_cast<float>(1 << tbits));
+    return am;
+}
+
+int launch_quantize(const void* k, const int64_t* strides, int dtype, int B, int Nk, int Nb, int rbits, int tbits,
+                    unsigned flags, uint8_t* codes, void* rscale, void* rmn, void* tscale, void* tmn,
+                    int cap, int off, hipStream_t st) {
+    dim3 grid(Nb, B * Nk), block(kQThreads);
+    const AngleMode am = angle_mode(dtype, tbits, flags);
+    const bool uniform = (flags & 2u) != 0;
     const bool packed6 = (flags & 4u) != 0;
     const bool libm = (flags & 8u) != 0;
 #define PQ_LAUNCH_QPL(T, U, P, L)                                                                                    \
     hipLaunchKernelGGL((quantize_kernel<T, U, P, L>), grid, block, 0, st, (const uint16_t*)k, strides[0], strides[1], \
                        strides[2], Nk, rbits, tbits, am, codes, (uint16_t*)rscale, (uint16_t*)rmn,                  \
-                       (uint16_t*)tscale, (uint16_t*)tmn, cap, off)
+                       (uint16_t*)tscale, (uint16_t*)tmn, cap, off, SealPages{})
 #define PQ_LAUNCH_QP(T, U, P)                                                                                        \
     do {                                                                                                             \
         if (libm) PQ_LAUNCH_QPL(T, U, P, true);                                                                      \
@@ -625,6 +640,23 @@ int launch_quantize(const void* k, const int64_t* strides, int dtype, int B, int
 #undef PQ_LAUNCH_QP
 #undef PQ_LAUNCH_QPL
     return static_cast<int>(hipGetLastError());
+}
+
+int launch_seal_pages(const void* keys, const SealPages& pages, int dtype, int B, int Nk, int rbits, int tbits, unsigned flags, uint8_t* codes, void* rscale,
+                      void* rmn, void* tscale, void* tmn, hipStream_t st) {
+    const AngleMode am = angle_mode(dtype, tbits, flags);
+    auto launch = [&](auto T, auto PK6, auto LIBM) {
+        hipLaunchKernelGGL((quantize_kernel<decltype(T), false, decltype(PK6)::value, decltype(LIBM)::value, true>), dim3(pages.Wo, B * Nk), dim3(kQThreads), 0, st,
+                           static_cast<const uint16_t*>(keys), 0, 0, kHeadDim, Nk, rbits, tbits, am, codes, static_cast<uint16_t*>(rscale),
+                           static_cast<uint16_t*>(rmn), static_cast<uint16_t*>(tscale), static_cast<uint16_t*>(tmn), 0, 0, pages);
+        return static_cast<int>(hipGetLastError());
+    };
+    const bool packed6 = (flags & 4u) != 0, libm = (flags & 8u) != 0;
+    auto by_flags = [&](auto T) {
+        if (packed6) return libm ? launch(T, std::true_type{}, std::true_type{}) : launch(T, std::true_type{}, std::false_type{});
+        return libm ? launch(T, std::false_type{}, std::true_type{}) : launch(T, std::false_type{}, std::false_type{});
+    };
+    return dtype == 0 ? by_flags(F16{}) : by_flags(BF16{});
 }
 
 }  // namespace pq

@@ -1,0 +1,244 @@
+"""A paged polar key cache (include/polarquant_paged.h): pages of 128 tokens that sequences hold through tables, rows into them, attention of new
+tokens over them, and pages out of the tables by the attention they receive.
+
+A step of a server, for each layer: `qk_norm_rope_append` writes the new tokens' keys and values, `paged_attention` reads all of them, and
+`seal_pages` turns the keys of pages that are full into polar codes.  Where the cache has to shrink, `page_weights` says what each page received
+and `evict_pages` closes the tables up without the pages that received least.
+
+A chunk may be one token or many, and sequences of a call need not agree in anything.  The reference takes one new token at a time over one contiguous
+cache (models/modeling_llama_polar.py:61-101).
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional, Tuple
+
+import torch
+
+from . import _ffi
+from ._ffi import calls as _calls
+from .attention import _num_cus
+from .kernel4group import _dtype_code, _on_device, _stream_ptr
+
+PAGE = 128
+
+
+def _gpu(t: torch.Tensor):
+    if not t.is_cuda:
+        raise RuntimeError("polarquant_amd: the paged cache's ops need tensors on the GPU (no CPU fallback)")
+
+
+def _refuse(condition: bool, message: str, *args):
+    if condition:
+        raise ValueError("polarquant_amd: " + message % args)
+
+
+class PagePool:
+    """One layer's physical pages: keys [open pages, Nk, 128, 128] (half-precision rows), values [pages, Nk, 128, 128], and of sealed pages codes [pages, Nk,
+    128, 64] (48: packed 6-bit codes) with rscale, rmn, tscale, tmn [pages, Nk, 1, 64].  Pages and heads may lie apart at any stride that is a multiple
+    of 8 elements.  Without codes every page is open."""
+
+    def __init__(self, keys: torch.Tensor, values: torch.Tensor, codes: Optional[torch.Tensor] = None, rscale: Optional[torch.Tensor] = None,
+                 rmn: Optional[torch.Tensor] = None, tscale: Optional[torch.Tensor] = None, tmn: Optional[torch.Tensor] = None, rbits: int = 4, tbits: int = 4):
+        self.keys, self.values, self.codes, self.meta, self.rbits, self.tbits = keys, values, codes, (rscale, rmn, tscale, tmn), rbits, tbits
+        _gpu(keys)
+        self.dtype, self.device, self.n_kv_heads, self.dt = keys.dtype, keys.device, keys.shape[1], _dtype_code(keys)
+
+        def part(t, name, width, dtype):
+            _refuse(t.dim() != 4 or t.shape[1] != self.n_kv_heads or tuple(t.shape[2:]) != (PAGE if width != 64 or name == "codes" else 1, width),
+                    "%s must be [pages, %d, .., %d], not %s", name, self.n_kv_heads, width, tuple(t.shape))
+            _refuse(t.dtype != dtype or t.device != self.device, "%s must be %s on %s", name, dtype, self.device)
+            _refuse(t.stride(3) != 1 or (t.shape[2] > 1 and t.stride(2) != width), "a page's rows of %s must follow each other", name)
+            return t.stride(0), t.stride(1)
+        key, value = part(keys, "keys", 128, self.dtype), part(values, "values", 128, self.dtype)
+        code = meta = (0, 0)
+        if codes is not None:
+            _refuse(any(m is None for m in self.meta), "codes need the constants of their groups")
+            code = part(codes, "codes", codes.shape[-1] if codes.dim() == 4 and codes.shape[-1] == 48 else 64, torch.uint8)
+            strides = [part(m, "a group's constants", 64, self.dtype) for m in self.meta]
+            meta = strides[0]
+            _refuse(any(s != meta for s in strides) or any(m.shape != rscale.shape for m in self.meta) or rscale.shape[0] != codes.shape[0],
+                    "the constants of a group must lie alike, a group a page of codes")
+        self.flags = _ffi.PQ_CODES_PACKED6 if codes is not None and codes.shape[-1] == 48 else 0
+        self.layout = (*key, *value, *code, *meta, keys.shape[0], values.shape[0], 0 if codes is None else codes.shape[0])
+
+    @classmethod
+    def empty(cls, n_pages: int, n_open: int, n_kv_heads: int, dtype: torch.dtype, device, rbits: int = 4, tbits: int = 4, packed: bool = False) -> "PagePool":
+        """A pool of `n_pages` pages, `n_open` of which can be open at a time."""
+        def new(*shape, kind=dtype):
+            return torch.zeros(shape, dtype=kind, device=device)
+        return cls(new(n_open, n_kv_heads, PAGE, 128), new(n_pages, n_kv_heads, PAGE, 128), new(n_pages, n_kv_heads, PAGE, 48 if packed else 64, kind=torch.uint8),
+                   *(new(n_pages, n_kv_heads, 1, 64) for _ in range(4)), rbits=rbits, tbits=tbits)
+
+
+class PageBatch:
+    """The sequences of a call: q_start int32 [B + 1] (sequence b's new tokens are packed rows q_start[b] .. q_start[b + 1] - 1), kv_len int32 [B] (tokens it holds,
+    the new ones last), n_sealed int32 [B] (leading pages whose keys are codes; None: none), pages int32 [B, W] (physical page of each logical one),
+    open_pages int32 [B, Wo] (physical pages of the keys of logical pages n_sealed, n_sealed + 1, ..).  All on the device; `max_q` and `max_kv` bound the new
+    tokens and the tokens of a sequence.  value_pages: the values' physical pages where they are other ones than the codes'.  A page that is not in the
+    pool (-1) does not exist: nothing is read from it or written to it."""
+
+    def __init__(self, q_start: Optional[torch.Tensor], kv_len: torch.Tensor, n_sealed: Optional[torch.Tensor], pages: torch.Tensor,
+                 open_pages: Optional[torch.Tensor], max_q: int, max_kv: int, value_pages: Optional[torch.Tensor] = None):
+        self.q_start, self.kv_len, self.n_sealed, self.pages, self.open_pages = q_start, kv_len, n_sealed, pages, open_pages
+        self.max_q, self.max_kv, self.value_pages = int(max_q), int(max_kv), pages if value_pages is None else value_pages
+        _gpu(kv_len)
+        self.device, self.size, self.width = kv_len.device, kv_len.numel(), pages.shape[-1]
+        self.open_width = 0 if open_pages is None else open_pages.shape[-1]
+        B = self.size
+        for t, shape in ((q_start, (B + 1,)), (kv_len, (B,)), (n_sealed, (B,)), (pages, (B, self.width)), (self.value_pages, (B, self.width)),
+                         (open_pages, (B, self.open_width))):
+            _refuse(t is not None and (t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != self.device),
+                    "counts and pages of a batch of %d must be contiguous int32 tensors on %s, %d pages wide", B, self.device, self.width)
+        _refuse(not 0 < self.max_kv <= PAGE * self.width, "max_kv must be within the %d pages of the table", self.width)
+
+
+def _heads(t: torch.Tensor, name: str, n: Optional[int] = None) -> Tuple[torch.Tensor, int, int, int]:
+    """Rows [T, n * 128] or [T, n, 128] as they lie -> (tensor, row stride, T, n); copied where the kernels could not read them."""
+    T, width = t.shape[0], t.shape[-1] if t.dim() == 2 else t.shape[1] * t.shape[2]
+    _refuse(t.dim() not in (2, 3) or (t.dim() == 3 and t.shape[2] != 128) or width % 128 != 0 or (n is not None and width != n * 128), "%s must be [T, heads, 128]", name)
+    row = t.stride(0)
+    if t.stride(-1) != 1 or (t.dim() == 3 and t.shape[1] > 1 and t.stride(1) != 128) or row % 8 or t.data_ptr() % 16 or (T > 1 and row < width):
+        t = t.contiguous().clone() if t.data_ptr() % 16 else t.contiguous()
+        row = width
+    return t, row if T > 1 else width, T, width // 128
+
+
+def _same(pool: PagePool, batch: PageBatch, *ts):
+    _refuse(batch.device != pool.device or any(t is not None and t.device != pool.device for t in ts), "tensors must be on the pool's device, %s", pool.device)
+    _refuse(batch.q_start is None, "the batch does not say which rows are whose (q_start)")
+
+
+def _mask(mask: Optional[torch.Tensor], batch: PageBatch):
+    if mask is None:
+        return None, 0
+    _refuse(mask.dim() != 2 or mask.shape[0] != batch.size or mask.shape[1] < batch.max_kv, "attention_mask must be [%d, >= %d]", batch.size, batch.max_kv)
+    mask = mask if mask.dtype == torch.uint8 else (mask != 0).to(torch.uint8)
+    mask = mask if mask.stride(1) == 1 and mask.stride(0) >= mask.shape[1] else mask.contiguous()
+    return mask, mask.stride(0)
+
+
+def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pool: PagePool, batch: PageBatch,
+                        q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                        positions: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """q [T, N * 128], k, v [T, Nk * 128] (projection outputs of the new tokens, packed; they may be slices of one) -> rotated queries [T, N, 128]; keys and
+    values go to their pages.  q_norm, k_norm [128]: queries, keys are first normed over each head's channels (None: not).  cos, sin [rows, 128]: the
+    table; a token's row is its place in its sequence, or positions[t] (int32 [T]: a sequence from which pages were evicted has its own); beyond
+    the table the nearest.  All in float32, rounded once.  Rows from q_start[-1] on are left as `out` has them."""
+    _gpu(q)
+    _same(pool, batch, q, k, v, cos, sin, q_norm, k_norm, positions, out)
+    Nk = pool.n_kv_heads
+    q, q_row, T, N = _heads(q, "q")
+    k, k_row, Tk, _ = _heads(k, "k", Nk)
+    v, v_row, Tv, _ = _heads(v, "v", Nk)
+    _refuse(Tk != T or Tv != T or N % Nk != 0, "q, k and v must have as many rows, and whole groups of heads")
+    for t in (k, v, cos, sin, q_norm, k_norm):
+        _refuse(t is not None and t.dtype != pool.dtype, "q, k, v, angles and norms must be %s", pool.dtype)
+    _refuse(q.dtype != pool.dtype, "q must be %s", pool.dtype)
+    _refuse(cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] != 128, "cos and sin must be [rows, 128]")
+    cos, sin = cos.contiguous(), sin.contiguous()
+    for t in (q_norm, k_norm):
+        _refuse(t is not None and (t.numel() != 128 or not t.is_contiguous()), "norms must be [128]")
+    _refuse(positions is not None and (positions.dtype != torch.int32 or positions.numel() != T or not positions.is_contiguous()), "positions must be int32 [T]")
+    if out is None:
+        out = _calls.empty(q, 0, T, N, 128)
+    _refuse(out.dtype != pool.dtype or tuple(out.shape) != (T, N, 128) or not out.is_contiguous(), "out must be a contiguous [%d, %d, 128]", T, N)
+    with _on_device(pool.device):
+        rc = _ffi.paged_lib().call.pq_paged_append(q, q_row, k, k_row, v, v_row, cos, sin, cos.shape[0], positions, q_norm, k_norm, float(eps), out, pool.keys,
+                                                   pool.values, pool.layout, batch.q_start, batch.kv_len, batch.n_sealed, batch.value_pages, batch.open_pages,
+                                                   batch.width, batch.open_width, T, batch.size, N, Nk, min(batch.max_q, T), batch.max_kv, pool.dt,
+                                                   _stream_ptr(pool.device))
+    _ffi.check(rc, "pq_paged_append")
+    return out
+
+
+def seal_pages(pool: PagePool, batch: PageBatch, eager_gpu: bool = False) -> None:
+    """Makes polar codes of the keys of every open page that its sequence fills, in the next sealed pages' place: as `quantize_and_pack_nbit` does, bit for bit.
+    The next call's batch counts kv_len // 128 pages as sealed, and its open_pages begin behind them."""
+    _refuse(pool.codes is None, "a pool without codes has no sealed pages")
+    _refuse(batch.device != pool.device or batch.open_pages is None, "the batch must be on %s and have open pages", pool.device)
+    with _on_device(pool.device):
+        rc = _ffi.lib().call.pq_seal_pages(pool.keys, pool.layout, pool.codes, *pool.meta, batch.kv_len, batch.n_sealed, batch.pages, batch.open_pages, batch.width,
+                                           batch.open_width, batch.size, pool.n_kv_heads, pool.rbits, pool.tbits, pool.dt,
+                                           pool.flags | (_ffi.PQ_EAGER_GPU if eager_gpu else 0), _stream_ptr(pool.device))
+    _ffi.check(rc, "pq_seal_pages")
+
+
+def paged_attention(q: torch.Tensor, pool: PagePool, batch: PageBatch, attention_mask: Optional[torch.Tensor] = None, sm_scale: Optional[float] = None,
+                    return_lse: bool = False, n_splits: Optional[int] = None, workspace: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None):
+    """q [T, N, 128] (rotated queries of the new tokens, packed) -> [T, N, 128]: each attends to its sequence's keys up to its own.  attention_mask [B, >=
+    max_kv] of {0, 1}: keys that are not there.  A row without a key is zero.  return_lse: also float32 [T, N], the natural logarithm of each row's sum of
+    exponentials (for `page_weights`).  The context is cut into up to `n_splits` slices through `workspace` (float32, of
+    paged_workspace_bytes(T, N, n_splits); by default memory of this call alone, so calls of several streams and graphs do not meet)."""
+    _gpu(q)
+    _same(pool, batch, q, attention_mask, workspace, out)
+    q, q_row, T, N = _heads(q, "q")
+    _refuse(q.dtype != pool.dtype or N % pool.n_kv_heads != 0, "q must be %s, with a multiple of %d heads", pool.dtype, pool.n_kv_heads)
+    mask, mask_row = _mask(attention_mask, batch)
+    lib, max_q, cus = _ffi.paged_lib().call, min(batch.max_q, T), _num_cus(pool.device)
+    if n_splits is None:
+        n_splits = lib.pq_paged_attn_plan(batch.size, N, pool.n_kv_heads, max_q, batch.max_kv, cus)
+    need = lib.pq_paged_attn_workspace_bytes(T, N, n_splits)
+    if workspace is None:
+        workspace = _calls.empty(q, 3, need // 4) if need else None
+    else:
+        _refuse(workspace.dtype != torch.float32 or not workspace.is_contiguous() or workspace.numel() * 4 < need, "workspace must be float32 with %d bytes", need)
+    if out is None:
+        out = _calls.empty(q, 0, T, N, 128)
+    _refuse(out.dtype != pool.dtype or tuple(out.shape) != (T, N, 128) or not out.is_contiguous(), "out must be a contiguous [%d, %d, 128]", T, N)
+    lse = _calls.empty(q, 3, T, N) if return_lse else None
+    with _on_device(pool.device):
+        rc = lib.pq_paged_attn(q, q_row, pool.keys, pool.values, pool.codes, *pool.meta, pool.layout, batch.q_start, batch.kv_len, batch.n_sealed, batch.pages,
+                               batch.value_pages, batch.open_pages, batch.width, batch.open_width, mask, mask_row, out, lse, T, batch.size, N, pool.n_kv_heads,
+                               max_q, batch.max_kv, pool.rbits, pool.tbits, float(1.0 / math.sqrt(128) if sm_scale is None else sm_scale), n_splits, cus, workspace,
+                               need, pool.dt, pool.flags, _stream_ptr(pool.device))
+    _ffi.check(rc, "pq_paged_attn")
+    return (out, lse) if return_lse else out
+
+
+def paged_workspace_bytes(T: int, N: int, n_splits: int) -> int:
+    return _ffi.paged_lib().call.pq_paged_attn_workspace_bytes(T, N, n_splits)
+
+
+def page_weights(q: torch.Tensor, lse: torch.Tensor, pool: PagePool, batch: PageBatch, onto: Optional[torch.Tensor] = None,
+                 attention_mask: Optional[torch.Tensor] = None, sm_scale: Optional[float] = None) -> torch.Tensor:
+    """The attention weight that the rows of q [T, N, 128] give to each page, summed over rows, tokens and a KV head's query heads: float32 [B, Nk, W], plus
+    `onto`.  lse [T, N] as `paged_attention` returns it for the same q, mask and scale; a row of -inf gives none."""
+    _gpu(q)
+    _same(pool, batch, q, lse, onto, attention_mask)
+    q, q_row, T, N = _heads(q, "q")
+    _refuse(q.dtype != pool.dtype or N % pool.n_kv_heads != 0, "q must be %s, with a multiple of %d heads", pool.dtype, pool.n_kv_heads)
+    _refuse(lse.dtype != torch.float32 or tuple(lse.shape) != (T, N) or not lse.is_contiguous(), "lse must be a contiguous float32 [%d, %d]", T, N)
+    shape = (batch.size, pool.n_kv_heads, batch.width)
+    _refuse(onto is not None and (onto.dtype != torch.float32 or tuple(onto.shape) != shape or not onto.is_contiguous()), "onto must be float32 %s", shape)
+    mask, mask_row = _mask(attention_mask, batch)
+    out = _calls.empty(q, 3, *shape)
+    with _on_device(pool.device):
+        rc = _ffi.paged_lib().call.pq_paged_weights(q, q_row, lse, pool.keys, pool.codes, *pool.meta, pool.layout, batch.q_start, batch.kv_len, batch.n_sealed,
+                                                    batch.pages, batch.value_pages, batch.open_pages, batch.width, batch.open_width, mask, mask_row, onto, out, T,
+                                                    batch.size, N, pool.n_kv_heads, min(batch.max_q, T), batch.max_kv, pool.rbits, pool.tbits,
+                                                    float(1.0 / math.sqrt(128) if sm_scale is None else sm_scale), pool.dt, pool.flags, _stream_ptr(pool.device))
+    _ffi.check(rc, "pq_paged_weights")
+    return out
+
+
+def evict_pages(weights: torch.Tensor, batch: PageBatch, keep: int, sinks: int = 1) -> Tuple[PageBatch, torch.Tensor, torch.Tensor]:
+    """Leaves each sequence at most `keep` sealed pages: its first `sinks`, and of the others those of the largest weight (the sum over the KV heads of weights
+    [B, Nk, W]; the earlier of equals).  Open pages stay.  -> the batch with its tables closed up in order (kv_len less the evicted tokens, q_start as
+    before), the weights likewise, and the evicted physical pages int32 [B, W], -1 behind them.  The keys keep the rotation of the positions they
+    were written at: later tokens of the sequence need `positions` of their own."""
+    _gpu(weights)
+    B, W = batch.size, batch.width
+    _refuse(weights.dtype != torch.float32 or weights.dim() != 3 or (weights.shape[0], weights.shape[2]) != (B, W) or not weights.is_contiguous()
+            or weights.device != batch.device, "weights must be a contiguous float32 [%d, Nk, %d] on %s", B, W, batch.device)
+    _refuse(batch.n_sealed is None, "the batch has no sealed pages")
+    _refuse(batch.value_pages is not batch.pages, "pages whose values lie elsewhere cannot be evicted")
+    _refuse(W > _ffi.PQ_EVICT_MAX_PAGES, "tables of more than %d pages cannot be evicted from", _ffi.PQ_EVICT_MAX_PAGES)
+    _refuse(not 0 <= sinks <= keep or keep < 1, "keep must be at least 1 and at least sinks")
+    pages, freed, n_sealed, kv_len = (_calls.empty(weights, 2, *s) for s in ((B, W), (B, W), (B,), (B,)))
+    left = _calls.empty(weights, 3, *weights.shape)
+    with _on_device(batch.device):
+        rc = _ffi.paged_lib().call.pq_evict_pages(weights, batch.pages, batch.n_sealed, batch.kv_len, B, weights.shape[1], W, keep, sinks, pages, n_sealed, kv_len,
+                                                  left, freed, _stream_ptr(batch.device))
+    _ffi.check(rc, "pq_evict_pages")
+    return PageBatch(batch.q_start, kv_len, n_sealed, pages, batch.open_pages, batch.max_q, batch.max_kv), left, freed

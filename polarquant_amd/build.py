@@ -37,7 +37,7 @@ LAYER_UNITS = {
     "latent": [("pq_latent_attn.hip", (), ""), ("pq_latent_norm.hip", (), ""), ("pq_latent_capi.hip", (), "")],
     "recurrent": [("pq_window_attn.hip", (), ""), ("pq_recurrent_chunk.hip", (), ""), ("pq_recurrent.hip", (), ""), ("pq_recurrent_token.hip", (), ""),
                   ("pq_recurrent_capi.hip", (), "")],
-    "paged": [("pq_paged_token.hip", (), ""), ("pq_paged_weights.hip", (), ""), ("pq_paged_rows.hip", (), ""), ("pq_paged_capi.hip", (), "")],
+    "paged": [("pq_paged_chunk.hip", (), ""), ("pq_paged_token.hip", (), ""), ("pq_paged_weights.hip", (), ""), ("pq_paged_rows.hip", (), ""), ("pq_paged_capi.hip", (), "")],
 }
 LAYER_LIBS = {name: os.path.join(HERE, "libpolarquant_%s.so" % name) for name in LAYER_UNITS}
 # measurement aids (a plain streaming read, the attention kernel's loads without its arithmetic): a library of

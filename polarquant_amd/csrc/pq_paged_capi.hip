@@ -173,7 +173,9 @@ int pq_paged_attn(const void* q, int64_t q_row, const void* keys, const void* va
     a.n_splits = n_splits;
     a.slots = 2 * (n_cus > 0 ? n_cus : 256);
     a.scale = scale;
-    return status(pq::launch_paged_token(a, dtype, (flags & PQ_CODES_PACKED6) != 0, static_cast<hipStream_t>(stream)));
+    const bool packed = (flags & PQ_CODES_PACKED6) != 0;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    return status(static_cast<int64_t>(max_q) * (N / Nk) <= pq::kPagedFewRows ? pq::launch_paged_token(a, dtype, packed, st) : pq::launch_paged_chunk(a, dtype, packed, st));
 }
 
 int pq_validate_paged_weights(const void* q, int64_t q_row, const float* lse, const void* keys, const uint8_t* codes, const void* rscale, const void* rmn,

@@ -1,0 +1,436 @@
+// Attention over the pages of a cache, for many query rows a sequence (a row: a new token and a query head).
+//
+// grid (KV heads, slices x row tiles, sequences), the row tiles that see most first.  Four wavefronts with 32 rows each over 64-key tiles of K and V that
+// are double-buffered in LDS; all query heads of a KV head share the tiles.  The transposed score tile S^T = K Q^T makes a row a lane, its softmax state a
+// register, and P^T the right operand of O^T = V^T P^T as it stands.
+//
+// Rows of values, and keys of open pages, go from memory to LDS directly, where the addresses that the lanes load from swizzle them so that 16 lanes' reads of 16
+// bytes, or 32 lanes' of 8, meet every bank.  Sealed keys are made from their codes by the four wavefronts together, 16 keys each, a tile ahead: a
+// lane has four pairs' radii in registers and looks their cos and sin up in a table of the page in LDS, 64 pairs x 16 bins of float16, made a page
+// ahead by all.  (More than 16 bins: cos and sin are evaluated for every code.)  A tile's codes are on their way to registers for a tile's time, a page's constants for
+// a page's.
+#include "pq_paged_device.h"
+
+namespace pq {
+
+constexpr int kChunkRows = 128, kChunkKeys = 64, kChunkTile = kChunkKeys * 256, kChunkTable = 4096, kChunkAhead = 4;
+
+template <typename T, bool PK6, bool TABLE>
+__global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttnArgs a) {
+    extern __shared__ __attribute__((aligned(1024))) uint8_t sm[];           // two tiles of K, two of V, two tables
+    const uint32_t lds0 = uniform(lds_addr(sm));
+    const int tid = threadIdx.x, lane = tid & 63, wv = uniform(tid >> 6), col = lane & 31, hi = lane >> 5, i16 = lane & 15, slot = lane >> 4;
+    const PagedCache& c = a.c;
+    const int b = blockIdx.z, h = blockIdx.x, slice = blockIdx.y % a.n_splits;
+    const PagedSequence s = own_sequence(c, b);
+    const int rep = c.N / c.Nk, rows = s.rows * rep, tiles = (rows + kChunkRows - 1) / kChunkRows, tile = tiles - 1 - static_cast<int>(blockIdx.y) / a.n_splits;
+    if (tile < 0) return;
+    const int pages = (s.kv + kPageTokens - 1) / kPageTokens;
+    const int per = pages_per_slice(c, pages, a.n_splits, a.slots, kChunkRows);
+    if (slice > 0 && slice * per >= pages) return;
+    const bool only = per >= pages;
+
+    const int row0 = tile * kChunkRows, last_row = row0 + kChunkRows - 1 < rows - 1 ? row0 + kChunkRows - 1 : rows - 1;
+    const int r = row0 + wv * 32 + col, rc = r < rows ? r : rows - 1, token = rc / rep;
+    const int limit = s.past + token;                                        // last key this row sees
+    const int wave_row = row0 + wv * 32 < rows - 1 ? row0 + wv * 32 : rows - 1, wave_end = wave_row + 31 < rows - 1 ? wave_row + 31 : rows - 1;
+    const int wave_first = uniform(s.past + wave_row / rep), wave_last = uniform(s.past + wave_end / rep), last_limit = uniform(s.past + last_row / rep);
+    const int p0 = slice * per, p1 = p0 + per < pages ? p0 + per : pages;
+    const int it0 = 2 * p0;
+    int it1 = 2 * p1 < (s.kv + kChunkKeys - 1) / kChunkKeys ? 2 * p1 : (s.kv + kChunkKeys - 1) / kChunkKeys;
+    if (const int seen = last_limit < 0 ? 0 : last_limit / kChunkKeys + 1; it1 > seen) it1 = seen;
+    const int border = 2 * s.sealed;                                         // tiles from here on are open
+
+    // ---- queries: in the order of a key's chunks of 16 bytes, of which this lane multiplies chunks 8 hi + i
+    const float scale2 = a.scale != 0.0f ? fabsf(a.scale) * kLog2e : 1.0f;
+    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u, keep = a.scale != 0.0f ? 0xffffffffu : 0u;
+    const uint16_t* qp = a.q + (s.first + token) * a.q_row + (h * rep + rc % rep) * 128;
+    u32x4_a q[8];
+    float row_scale = scale2;
+    auto masked = [&](u32x4_a w) { return u32x4_a{(w.x ^ flip) & keep, (w.y ^ flip) & keep, (w.z ^ flip) & keep, (w.w ^ flip) & keep}; };
+    auto load_for_sealed = [&]() {          // chunk c: channels 4 c .. 4 c + 3 and 64 + 4 c .. 64 + 4 c + 3
+        u32x4_a x[4], y[4];
+        static_for<4>([&](auto I) {
+            x[I] = *reinterpret_cast<const u32x4_a*>(qp + 32 * hi + 8 * I);
+            y[I] = *reinterpret_cast<const u32x4_a*>(qp + 64 + 32 * hi + 8 * I);
+        });
+        static_for<4>([&](auto I) {
+            const u32x4_a xm = masked(x[I]), ym = masked(y[I]);
+            q[2 * I] = u32x4_a{xm.x, xm.y, ym.x, ym.y};
+            q[2 * I + 1] = u32x4_a{xm.z, xm.w, ym.z, ym.w};
+        });
+        if constexpr (std::is_same<T, BF16>::value) {
+            float most = 0.0f;
+            static_for<8>([&](auto I) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const uint32_t w = q[I][j];
+                    most = fmaxf(most, fmaxf(fabsf(lo2f<T>(static_cast<uint16_t>(w & 0xffffu))), fabsf(lo2f<T>(static_cast<uint16_t>(w >> 16)))));
+                }
+            });
+            const int e = within(kHalfTop - exponent_above(both_halves_max(most)), -120, 120);
+            const float factor = __builtin_ldexpf(1.0f, e);
+            static_for<8>([&](auto I) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) q[I][j] = scaled_half<T>(q[I][j], factor);
+            });
+            row_scale = scale2 * __builtin_ldexpf(1.0f, -e);
+        }
+    };
+    auto load_for_open = [&]() {            // chunk c: channels 8 c .. 8 c + 7
+        static_for<8>([&](auto I) { q[I] = *reinterpret_cast<const u32x4_a*>(qp + 64 * hi + 8 * I); });
+        static_for<8>([&](auto I) { q[I] = masked(q[I]); });
+        row_scale = scale2;
+    };
+
+    // ---- what is on its way
+    struct Ids { int key, value; };
+    auto asked_ids = [&](int p, int& key, int& value) {                      // (as they lie in the tables: checked when they are taken)
+        const int pc = p < c.W ? p : c.W - 1;
+        value = c.value_pages[static_cast<int64_t>(b) * c.W + pc];
+        const int oc = p - s.sealed;
+        key = p < s.sealed ? c.pages[static_cast<int64_t>(b) * c.W + pc] : oc < c.Wo ? c.open_pages[static_cast<int64_t>(b) * c.Wo + oc] : -1;
+    };
+    auto taken_ids = [&](int p, int key, int value) {
+        const int k = uniform(key), v = uniform(value);
+        const bool there = static_cast<unsigned>(k) < static_cast<unsigned>(p < s.sealed ? c.codes.n : c.keys.n) && static_cast<unsigned>(v) < static_cast<unsigned>(c.values.n);
+        return Ids{there ? k : -1, there ? v : -1};
+    };
+    Ids now, next;                          // of the page of the tile that is computed, of the one behind it
+    int raw_key = -1, raw_value = -1;       // of the one behind that
+    uint32_t cw[PK6 ? 8 : 4] = {};          // codes of the tile behind the one that is made
+    uint2 raw_rs = make_uint2(0, 0), raw_rm = raw_rs, raw_ts = raw_rs, raw_tm = raw_rs;
+    float rs[4] = {}, of[4] = {}, ts[4] = {}, tm[4] = {};
+    float page_scale = 1.0f, page_scale_next = 1.0f;
+    uint8_t seen_byte = 1;                  // the mask's, of the tile behind the one that is asked for
+    const float angle_bits = 1.0f / static_cast<float>(1 << c.tbits);
+    const uint32_t angles4 = ((1u << c.tbits) - 1u) * 0x01010101u;
+
+    auto ask_mask = [&](int it) {
+        if (!a.mask) return;
+        const int key = it * kChunkKeys + lane;
+        seen_byte = a.mask[b * a.mask_row + (key < s.kv ? key : s.kv - 1)];
+    };
+    auto keys_there = [&](int it, const Ids& id) -> uint64_t {
+        if (id.key < 0) return 0;
+        const int n = s.kv - it * kChunkKeys;
+        uint64_t bits = n >= 64 ? ~uint64_t{0} : (uint64_t{1} << n) - 1;
+        if (a.mask) bits &= __ballot(seen_byte != 0);
+        return bits;
+    };
+    auto ask_codes = [&](int it, int page) {
+        const uint8_t* at = static_cast<const uint8_t*>(c.codes.at) + page * c.codes.page + h * c.codes.head;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int row = (it & 1) * kChunkKeys + 16 * wv + 4 * j + slot;
+            if constexpr (PK6) {
+                const uint32_t* w = reinterpret_cast<const uint32_t*>(at + row * 48);
+                const int d = (3 * i16) >> 2;
+                cw[2 * j] = w[d];
+                cw[2 * j + 1] = w[d < 11 ? d + 1 : 11];
+            } else {
+                cw[j] = *reinterpret_cast<const uint32_t*>(at + row * 64 + 4 * i16);
+            }
+        }
+    };
+    auto ask_constants = [&](int page) {
+        const int64_t at = page * c.meta.page + h * c.meta.head + 4 * i16;
+        raw_rs = *reinterpret_cast<const uint2*>(c.rscale + at);
+        raw_rm = *reinterpret_cast<const uint2*>(c.rmn + at);
+        raw_ts = *reinterpret_cast<const uint2*>(c.tscale + at);
+        raw_tm = *reinterpret_cast<const uint2*>(c.tmn + at);
+    };
+    auto fourth = [](const uint2& w, int k) { return lo2f<T>(static_cast<uint16_t>((k < 2 ? w.x : w.y) >> (16 * (k & 1)))); };
+    auto take_radii = [&]() {
+        float most = 0.0f;
+        const float top = static_cast<float>(1 << c.rbits);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            rs[k] = fourth(raw_rs, k);
+            of[k] = fourth(raw_rm, k);
+            most = fmaxf(most, __builtin_fmaf(fabsf(rs[k]), top, fabsf(of[k])));
+            of[k] = __builtin_fmaf(rs[k], 0.5f, of[k]);
+        }
+        most = fmaxf(most, __uint_as_float(row_rotate<8>(__float_as_uint(most))));
+        most = fmaxf(most, __uint_as_float(row_rotate<4>(__float_as_uint(most))));
+        most = fmaxf(most, __uint_as_float(row_rotate<2>(__float_as_uint(most))));
+        most = fmaxf(most, __uint_as_float(row_rotate<1>(__float_as_uint(most))));
+        const int e = within(kHalfTop - exponent_above(most), -120, 120);
+        const float factor = __builtin_ldexpf(1.0f, e);
+        page_scale_next = __builtin_ldexpf(1.0f, -e);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            rs[k] *= factor * angle_bits;                                    // (a radius code comes as a byte, above the angle's bits)
+            of[k] *= factor;
+            if constexpr (!TABLE) {
+                ts[k] = fourth(raw_ts, k) * kTurn;
+                tm[k] = __builtin_fmaf(ts[k], 0.5f, fourth(raw_tm, k) * kTurn);
+            }
+        }
+    };
+    auto make_table = [&](int p) {
+        if constexpr (TABLE) {
+            const int bin = tid >> 4;
+            const uint32_t at = lds0 + 4 * kChunkTile + (p & 1) * kChunkTable + (i16 * 16 + bin) * 4;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const float width = fourth(raw_ts, k) * kTurn;
+                *lds_ptr<lds_u32>(at + k * 1024) = cos_sin_half(__builtin_fmaf(static_cast<float>(bin) + 0.5f, width, fourth(raw_tm, k) * kTurn));
+            }
+        }
+    };
+    // this wavefront's 16 keys of a sealed tile, from cw
+    auto make_keys = [&](int it, uint32_t to) {
+        const uint32_t table = lds0 + 4 * kChunkTile + ((it >> 1) & 1) * kChunkTable + i16 * 64;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            uint32_t w;
+            if constexpr (PK6) w = unpack_codes6(static_cast<uint32_t>(((static_cast<uint64_t>(cw[2 * j + 1]) << 32) | cw[2 * j]) >> (8 * ((3 * i16) & 3))));
+            else w = cw[j];
+            float rad[4];
+            uint32_t cs[4];
+            uint32_t r4 = w & ~angles4;
+            if constexpr (TABLE) {
+                uint32_t a4 = (w & angles4) << 2;
+                asm volatile("" : "+v"(a4), "+v"(r4));
+#pragma unroll
+                for (int k = 0; k < 4; k++) cs[k] = *lds_ptr<lds_u32>(table + ((a4 >> (8 * k)) & 0xffu) + k * 1024);
+            } else {
+                const uint32_t a4 = w & angles4;
+#pragma unroll
+                for (int k = 0; k < 4; k++) cs[k] = cos_sin_half(__builtin_fmaf(static_cast<float>((a4 >> (8 * k)) & 0xffu), ts[k], tm[k]));
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) rad[k] = __builtin_fmaf(static_cast<float>((r4 >> (8 * k)) & 0xffu), rs[k], of[k]);
+            const int row = 16 * wv + 4 * j + slot;
+            *lds_ptr<lds_u32x4>(to + row * 256 + (i16 ^ (4 * j + slot)) * 16) = quad_of_pairs(rad, cs);
+        }
+    };
+    // rows to LDS; rows that are not there are copies of one that is, with weight zero
+    auto ask_rows = [&](const PageStream& from, int page, int it, uint64_t bits, uint32_t to, auto KEYS) {
+        const u32x4_a at = rows_at(static_cast<const uint16_t*>(from.at) + page * from.page + h * from.head + (it & 1) * (kChunkKeys * 128));
+        const int some = bits ? __builtin_ctzll(bits) : 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int row = 16 * wv + 4 * i + slot, chunk = decltype(KEYS)::value ? i16 ^ (4 * i + slot) : i16 ^ (slot << 2);
+            const int r = (bits >> row) & 1 ? row : some;
+            rows_to_lds(at, r * 256 + chunk * 16, to + (wv * 4 + i) * 1024);
+        }
+    };
+
+    floatx16_a o[4];
+    static_for<4>([&](auto I) {
+#pragma unroll
+        for (int j = 0; j < 16; j++) o[I][j] = 0.0f;
+    });
+    float m = kNone, l = 0.0f;
+    uint32_t ka[8], va[4];
+    static_for<8>([&](auto I) { ka[I] = lds0 + col * 256 + ((8 * hi + I) ^ (col & 15)) * 16; });
+    static_for<4>([&](auto I) {              // 16 lanes read 4 tokens x 16 channels and get them transposed
+        constexpr int i = decltype(I)::value;
+        const int row = 4 * hi + (i16 >> 2), chunk = 4 * i + 2 * (slot & 1) + ((lane & 3) >> 1);
+        va[i] = lds0 + 2 * kChunkTile + row * 256 + (chunk ^ ((row & 3) << 2)) * 16 + (lane & 1) * 8;
+    });
+
+    uint64_t bits = 0, bits_next = 0;
+    auto compute = [&](int it, auto BUF) {
+        constexpr int buf = decltype(BUF)::value;
+        const int key0 = it * kChunkKeys;
+        floatx16_a z[2];
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int j = 0; j < 16; j++) z[u][j] = 0.0f;
+        auto scores = [&](auto OF) {
+            using TQ = decltype(OF);
+            u32x4_a kf[kChunkAhead][2];
+            auto k_load = [&](auto I) {
+                constexpr int i = decltype(I)::value;
+                kf[i % kChunkAhead][0] = *lds_ptr<lds_u32x4>(ka[i] + buf * kChunkTile);
+                kf[i % kChunkAhead][1] = *lds_ptr<lds_u32x4>(ka[i] + buf * kChunkTile + 32 * 256);
+            };
+            static_for<kChunkAhead>(k_load);
+            static_for<8>([&](auto I) {
+                constexpr int i = decltype(I)::value;
+                z[0] = mma32<TQ>(kf[i % kChunkAhead][0], q[i], z[0]);
+                z[1] = mma32<TQ>(kf[i % kChunkAhead][1], q[i], z[1]);
+                if constexpr (i + kChunkAhead < 8) k_load(IC<i + kChunkAhead>{});
+            });
+        };
+        float f = row_scale;
+        if (std::is_same<T, F16>::value || it < border) scores(F16{});
+        else scores(T{});
+        if (it < border) f *= page_scale;
+        if (bits != ~uint64_t{0} || key0 + kChunkKeys - 1 > wave_first) {
+            const int last = limit - key0 - 4 * hi;
+            const uint64_t there = bits >> (4 * hi);
+            const uint32_t half[2] = {static_cast<uint32_t>(there), static_cast<uint32_t>(there >> 32)};
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int j = 0; j < 16; j++) {
+                    const int e = 8 * (j >> 2) + (j & 3);
+                    z[u][j] = 32 * u + e <= last && (half[u] >> e & 1) ? z[u][j] : -INFINITY;
+                }
+        }
+        float mx = fmaxf(z[0][0], z[1][0]);
+#pragma unroll
+        for (int j = 1; j < 16; j++) mx = fmaxf(fmaxf(mx, z[0][j]), z[1][j]);
+        mx = both_halves_max(mx) * f;
+        if (__any(mx > m)) {
+            const float mn = fmaxf(m, mx), al = exp2_hw(m - mn);
+            l *= al;
+            static_for<4>([&](auto I) {
+#pragma unroll
+                for (int j = 0; j < 16; j++) o[I][j] *= al;
+            });
+            m = mn;
+        }
+        // right operands of the four 16-token steps, each made beside the products of the one before it
+        u32x4_a p[2], vf[2][4];
+        float sum[2] = {0.0f, 0.0f};
+        auto v_load = [&](auto J, auto I) {
+            constexpr int j = decltype(J)::value, i = decltype(I)::value;
+            const uint32_t at = va[i] + buf * kChunkTile + j * 16 * 256;
+            const u32x2_a w0 = __builtin_bit_cast(u32x2_a, __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_ptr<lds_short4>(at)));
+            const u32x2_a w1 = __builtin_bit_cast(u32x2_a, __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_ptr<lds_short4>(at + 8 * 256)));
+            vf[j & 1][i] = u32x4_a{w0.x, w0.y, w1.x, w1.y};
+        };
+        auto weights = [&](auto J, auto N) {                    // the Nth two of step J
+            constexpr int u = decltype(J)::value >> 1, n = decltype(N)::value, j = 8 * (decltype(J)::value & 1) + 2 * n;
+            const float e0 = exp2_hw(__builtin_fmaf(z[u][j], f, -m)), e1 = exp2_hw(__builtin_fmaf(z[u][j + 1], f, -m));
+            sum[0] += e0;
+            sum[1] += e1;
+            p[decltype(J)::value & 1][n] = pack_pair<T>(e0, e1);
+        };
+        static_for<4>([&](auto I) { v_load(IC<0>{}, I); });
+        static_for<4>([&](auto N) { weights(IC<0>{}, N); });
+        __builtin_amdgcn_sched_barrier(0);
+        static_for<4>([&](auto J) {
+            constexpr int j = decltype(J)::value;
+            static_for<4>([&](auto I) {
+                constexpr int i = decltype(I)::value;
+                o[i] = mma32<T>(vf[j & 1][i], p[j & 1], o[i]);
+                if constexpr (j < 3) {
+                    v_load(IC<j + 1>{}, I);
+                    weights(IC<j + 1>{}, I);
+                }
+                __builtin_amdgcn_sched_barrier(0);              // (left alone, the compiler makes all weights first)
+            });
+        });
+        l += sum[0] + sum[1];
+    };
+    auto step = [&](int it, auto BUF) {
+        constexpr int buf = decltype(BUF)::value;
+        const bool first_half = (it & 1) == 0;
+        const int p = it >> 1;
+        // what is taken here was asked for a step ago, except the constants of a page's radii, two
+        if (!first_half) {
+            const Ids after = taken_ids(p + 2, raw_key, raw_value);
+            if (it + 1 < it1 && it + 1 < border && next.key >= 0) take_radii();
+            now = next;                      // (the tile that is made now is the next page's)
+            next = after;
+            if (it + 3 < it1 && it + 3 < border && next.key >= 0) ask_constants(next.key);
+        } else {
+            if (it + 2 < it1 && it + 2 < border && next.key >= 0) make_table(p + 1);
+            asked_ids(p + 2, raw_key, raw_value);
+        }
+        if (it + 1 < it1) {
+            bits_next = keys_there(it + 1, now);
+            ask_mask(it + 2);
+            const bool sealed = it + 1 < border;
+            if (bits_next) {
+                ask_rows(c.values, now.value, it + 1, bits_next, lds0 + 2 * kChunkTile + (buf ^ 1) * kChunkTile, std::false_type{});
+                if (!sealed) ask_rows(c.keys, now.key, it + 1, bits_next, lds0 + (buf ^ 1) * kChunkTile, std::true_type{});
+                else make_keys(it + 1, lds0 + (buf ^ 1) * kChunkTile);
+            }
+            const int key = first_half ? next.key : now.key;                 // of tile it + 2
+            if (it + 2 < it1 && it + 2 < border && key >= 0) ask_codes(it + 2, key);
+        }
+        if (it == border && it > it0) load_for_open();
+        if (bits && it * kChunkKeys <= wave_last) compute(it, BUF);
+        rows_arrived();
+        __syncthreads();
+        bits = bits_next;
+        if (!first_half) page_scale = page_scale_next;
+    };
+
+    if (it0 < it1) {
+        int key, value;
+        asked_ids(p0, key, value);
+        asked_ids(p0 + 1, raw_key, raw_value);
+        ask_mask(it0);
+        if (it0 < border) load_for_sealed(); else load_for_open();
+        now = taken_ids(p0, key, value);
+        next = taken_ids(p0 + 1, raw_key, raw_value);
+        const bool sealed = it0 < border && now.key >= 0;
+        bits = keys_there(it0, now);
+        if (bits) {
+            ask_rows(c.values, now.value, it0, bits, lds0 + 2 * kChunkTile, std::false_type{});
+            if (it0 >= border) ask_rows(c.keys, now.key, it0, bits, lds0, std::true_type{});
+        }
+        ask_mask(it0 + 1);
+        if (sealed) {
+            ask_codes(it0, now.key);
+            ask_constants(now.key);
+            take_radii();
+            make_table(p0);
+        }
+        page_scale = page_scale_next;
+        __syncthreads();
+        if (sealed) {
+            if (bits) make_keys(it0, lds0);
+            if (it0 + 1 < it1) ask_codes(it0 + 1, now.key);
+        }
+        if (it0 + 2 < it1 && it0 + 2 < border && next.key >= 0) ask_constants(next.key);
+        rows_arrived();
+        __syncthreads();
+    }
+    for (int it = it0; it < it1; it += 2) {
+        step(it, IC<0>{});
+        if (it + 1 < it1) step(it + 1, IC<1>{});
+    }
+
+    l += __shfl_xor(l, 32);
+    if (r >= rows) return;
+    const size_t at = static_cast<size_t>(s.first + token) * c.N + h * rep + rc % rep;
+    if (only) {
+        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+        uint16_t* out = a.out + at * 128 + 4 * hi;
+        static_for<4>([&](auto I) {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                *reinterpret_cast<uint2*>(out + I * 32 + 8 * j) = make_uint2(pack_pair<T>(o[I][4 * j] * inv, o[I][4 * j + 1] * inv), pack_pair<T>(o[I][4 * j + 2] * inv, o[I][4 * j + 3] * inv));
+        });
+        if (a.lse && hi == 0) a.lse[at] = l > 0.0f ? (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f : -INFINITY;
+    } else {
+        float* out = a.partial + (at * a.n_splits + slice) * 128 + 4 * hi;
+        static_for<4>([&](auto I) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) *reinterpret_cast<float4*>(out + I * 32 + 8 * j) = make_float4(o[I][4 * j], o[I][4 * j + 1], o[I][4 * j + 2], o[I][4 * j + 3]);
+        });
+        if (hi == 0) *reinterpret_cast<float2*>(a.partial + static_cast<size_t>(c.T) * c.N * a.n_splits * 128 + 2 * (at * a.n_splits + slice)) = make_float2(m, l);
+    }
+}
+
+template <typename T, bool PK6, bool TABLE>
+static int launch_chunk(const PagedAttnArgs& a, hipStream_t st) {
+    constexpr int bytes = 4 * kChunkTile + (TABLE ? 2 * kChunkTable : 0);
+    const void* f = reinterpret_cast<const void*>(&paged_chunk_kernel<T, PK6, TABLE>);
+    if (const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, bytes); e != hipSuccess) return static_cast<int>(e);
+    const int tiles = (a.max_q * (a.c.N / a.c.Nk) + kChunkRows - 1) / kChunkRows;
+    hipLaunchKernelGGL((paged_chunk_kernel<T, PK6, TABLE>), dim3(a.c.Nk, tiles * a.n_splits, a.c.B), dim3(256), bytes, st, a);
+    const int err = static_cast<int>(hipGetLastError());
+    return err || a.n_splits == 1 ? err : launch_paged_merge(a, std::is_same<T, F16>::value ? 0 : 1, kChunkRows, st);
+}
+
+int launch_paged_chunk(const PagedAttnArgs& a, int dtype, bool packed, hipStream_t st) {
+    auto of = [&](auto T) {
+        using E = decltype(T);
+        if (packed) return launch_chunk<E, true, true>(a, st);
+        return a.c.tbits <= 4 ? launch_chunk<E, false, true>(a, st) : launch_chunk<E, false, false>(a, st);
+    };
+    return dtype == 0 ? of(F16{}) : of(BF16{});
+}
+
+}  // namespace pq

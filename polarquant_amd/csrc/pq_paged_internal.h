@@ -37,6 +37,7 @@ struct PagedAttnArgs {
     float scale;
 };
 int launch_paged_token(const PagedAttnArgs& a, int dtype, bool packed, hipStream_t st);
+int launch_paged_chunk(const PagedAttnArgs& a, int dtype, bool packed, hipStream_t st);
 int launch_paged_merge(const PagedAttnArgs& a, int dtype, int tile_rows, hipStream_t st);
 
 struct PagedWeightArgs {

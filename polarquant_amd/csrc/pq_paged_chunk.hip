@@ -348,7 +348,7 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttnArgs a) {
             if (it + 2 < it1 && it + 2 < border && key >= 0) ask_codes(it + 2, key);
         }
         if (it == border && it > it0) load_for_open();
-        if (bits && it * kChunkKeys <= wave_last) compute(it, BUF);
+        if (bits && it * kChunkKeys <= wave_last && row0 + wv * 32 < rows) compute(it, BUF);
         rows_arrived();
         __syncthreads();
         bits = bits_next;

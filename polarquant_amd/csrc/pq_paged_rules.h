@@ -4,10 +4,10 @@
 
 namespace pq {
 
-constexpr int kPagedFewRows = 32;             // rows a sequence that the kernel for few rows takes
+constexpr int kPagedFewRows = 16;             // rows a sequence that the kernel for few rows takes
 
 // rows of a workgroup of the kernel that a call of `rows` rows a sequence runs
-inline int paged_tile_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= kPagedFewRows ? 32 : 128; }
+inline int paged_tile_rows(int64_t rows) { return rows <= kPagedFewRows ? 16 : 128; }
 
 // Slices a sequence may be cut into: enough that two workgroups stand on every unit, twice as many where sequences can differ (the device deals
 // the slices out by the lengths it finds; a workgroup without one ends at once), no more than there are pages.

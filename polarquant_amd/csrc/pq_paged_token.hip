@@ -1,10 +1,13 @@
 // Attention over the pages of a cache, for few query rows a sequence (a row: a new token and a query head), and the merge of its slices.
 //
 // grid (KV heads, slices x row tiles, sequences).  A workgroup owns 16 NQ rows and a slice of whole pages; its four wavefronts divide the slice's
-// blocks of 32 tokens among them and run on their own until their states are joined in LDS, so nothing waits at a barrier.  As in the prompt
-// kernel the score tile is transposed, S^T = K Q^T: a row is a lane, its softmax state a register, and the weights are the right operand of
-// O^T = V^T P^T as they stand.  The left operand of S^T has a key's row in a lane, 16 pairs in each of the four lanes of a key: what a lane
-// loads of the codes (16 bytes) becomes its operand without passing through LDS.
+// blocks of 32 tokens among them and run on their own until their states are joined in LDS, so nothing waits at a barrier.  The score tile is transposed, S^T = K
+// Q^T: a row is a lane, its softmax state a register, and the weights are the right operand of O^T = V^T P^T as they stand.
+//
+// Everything comes straight to registers.  The left operand of S^T has a key's row in four lanes, 16 pairs in each: what a lane loads of the codes, 16 bytes, becomes its
+// operand in place.  Of the values a lane loads 8 channels of 8 tokens, which v_perm turns into the operands of eight products, channel 8 (lane % 16) + i in the
+// i-th.  Two sets of registers take turns: a block's codes are asked for when those of the block two before it have been used, its values likewise, so
+// up to two blocks, 20 KB a wavefront, are on their way, and all waits are the compiler's.
 //
 // Angles go through a table of cos and sin in LDS, 64 pairs x 16 bins of float16, which a wavefront makes once a page: word (pair % 16) 64 +
 // (pair / 16) 16 + bin, so that the lanes of a lookup, four pairs and sixteen keys, meet a bank only with a lane that wants the same word.
@@ -13,9 +16,20 @@
 
 namespace pq {
 
-constexpr int kTokenBlock = 32, kTokenValues = kTokenBlock * 256, kTokenTable = 4096, kTokenWave = 2 * kTokenValues + kTokenTable;
+constexpr int kTokenBlock = 32, kTokenTable = 4096;
+constexpr int kStream = 2;                    // every key and value is read once: the loads do not displace what the caches could keep
 
-template <typename T, int NQ, bool PK6, bool TABLE>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t stream_at(const void* p, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, static_cast<int>(bytes), 0x00020000);
+}
+__device__ __forceinline__ u32x4_a stream16(__amdgpu_buffer_rsrc_t r, uint32_t lane_offset, int offset) {
+    return __builtin_bit_cast(u32x4_a, __builtin_amdgcn_raw_buffer_load_b128(r, static_cast<int>(lane_offset), offset, kStream));
+}
+
+// bytes of LDS: tables, in whose place the wavefronts' states are joined
+template <int NQ> constexpr int token_lds() { return 4 * (16 * NQ * 512 + 16 * NQ * 8); }
+
+template <typename T, int NQ, bool PK6, bool TABLE, bool MASK>
 __global__ __launch_bounds__(256, 2) void paged_token_kernel(PagedAttnArgs a) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t sm[];
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, g = lane >> 4;
@@ -28,8 +42,7 @@ __global__ __launch_bounds__(256, 2) void paged_token_kernel(PagedAttnArgs a) {
     const int per = pages_per_slice(c, pages, a.n_splits, a.slots, 16 * NQ);
     if (slice > 0 && slice * per >= pages) return;
     const bool only = per >= pages;
-
-    const uint32_t lds0 = uniform(lds_addr(sm) + wv * kTokenWave), table = lds0 + 2 * kTokenValues;
+    const uint32_t table = uniform(lds_addr(sm) + wv * kTokenTable);
 
     // this lane's rows, the keys they see, and their queries: 16 channels from 16 g on and 16 from 64 + 16 g on, which is the order of a key's pairs
     const float scale2 = a.scale != 0.0f ? fabsf(a.scale) * kLog2e : 1.0f;
@@ -57,18 +70,17 @@ __global__ __launch_bounds__(256, 2) void paged_token_kernel(PagedAttnArgs a) {
             q[n][3] = u32x4_a{w[1].z, w[1].w, w[3].z, w[3].w};
         }
     };
-    const int first_limit = s.past + row0 / rep;                             // of the tile's rows: the least, the largest
-    const int last_row = row0 + 16 * NQ - 1 < rows - 1 ? row0 + 16 * NQ - 1 : rows - 1, last_limit = s.past + last_row / rep;
+    const int first_limit = uniform(s.past + row0 / rep);                    // of the tile's rows: the least, the largest
+    const int last_row = row0 + 16 * NQ - 1 < rows - 1 ? row0 + 16 * NQ - 1 : rows - 1, last_limit = uniform(s.past + last_row / rep);
 
     // this wavefront's blocks
     int blocks = (s.kv + kTokenBlock - 1) / kTokenBlock;
     const int p0 = slice * per, p1 = p0 + per < pages ? p0 + per : pages;
-    const int mine = (4 * (p1 - p0) + 3) / 4;
-    int blk0 = 4 * p0 + wv * mine, blk1 = blk0 + mine;
-    if (blk1 > 4 * p1) blk1 = 4 * p1;
+    const int mine = p1 - p0;                 // (a quarter of four blocks a page)
+    const int blk0 = 4 * p0 + wv * mine;
     const int seen = last_limit < 0 ? 0 : last_limit / kTokenBlock + 1;
     if (blocks > seen) blocks = seen;
-    if (blk1 > blocks) blk1 = blocks;
+    const int blk1 = blk0 + mine < blocks ? blk0 + mine : blocks;
     const int border = 4 * s.sealed;
 
     floatx4_a o[NQ][8];
@@ -80,104 +92,101 @@ __global__ __launch_bounds__(256, 2) void paged_token_kernel(PagedAttnArgs a) {
 #pragma unroll
         for (int i = 0; i < 8; i++) o[n][i] = floatx4_a{0.0f, 0.0f, 0.0f, 0.0f};
     }
-
-    // where 16 lanes read 4 tokens x 16 channels of the values and get them transposed, and what lane's 16 bytes go there: pieces of 16 bytes are
-    // swizzled by the token so that 8 tokens' reads of 32 bytes meet every bank once
-    uint32_t tops[8];                                                        // of channel tile i: chunks 2 i and 2 i + 1
-    {
-        const int row = 4 * g + (r16 >> 2);
-#pragma unroll
-        for (int i = 0; i < 8; i++) tops[i] = lds0 + row * 256 + ((2 * i + ((lane & 3) >> 1)) ^ ((row & 7) << 1)) * 16 + (lane & 1) * 8;
-    }
-
     const float rest = 1.0f / static_cast<float>(1 << c.tbits);
     const uint32_t angles4 = ((1u << c.tbits) - 1u) * 0x01010101u;
+    const uint32_t value_lane = g * 1024 + r16 * 16;                         // tokens 4 g + j and 16 + 4 g + j, channels 8 r16 ..
 
     auto walk = [&](auto SEALED, int blk, const int end) {
         constexpr bool sealed = decltype(SEALED)::value;
         using TQ = std::conditional_t<sealed, F16, T>;
         if (blk >= end) return;
+        // physical pages of 64 logical ones, a lane each
+        int window = -1, key_ids = -1, value_ids = -1;
+        auto look_up = [&](int p) {
+            window = p;
+            const int at = p + lane;
+            const bool in = at < c.W && (sealed ? at < s.sealed : at - s.sealed < c.Wo);
+            const int ac = in ? at : p;
+            const int k = sealed ? c.pages[static_cast<int64_t>(b) * c.W + ac] : in ? c.open_pages[static_cast<int64_t>(b) * c.Wo + (ac - s.sealed)] : -1;
+            const int v = c.value_pages[static_cast<int64_t>(b) * c.W + ac];
+            const bool there = static_cast<unsigned>(k) < static_cast<unsigned>(sealed ? c.codes.n : c.keys.n) && static_cast<unsigned>(v) < static_cast<unsigned>(c.values.n);
+            key_ids = in && there ? k : -1;
+            value_ids = v;
+        };
+        look_up(blk >> 2);
         load_queries();
         float sc[NQ], page_scale = 1.0f;
-#pragma unroll
-        for (int n = 0; n < NQ; n++) {
-            sc[n] = scale2;
-            if constexpr (sealed && std::is_same<T, BF16>::value) {
-                float most = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const uint32_t w = q[n][i][j];
-                        most = fmaxf(most, fmaxf(fabsf(lo2f<T>(static_cast<uint16_t>(w & 0xffffu))), fabsf(lo2f<T>(static_cast<uint16_t>(w >> 16)))));
-                    }
-                most = both_halves_max(both_rows_max(most));
-                const int e = exponent_above(most);
-                const float factor = __builtin_ldexpf(1.0f, within(kHalfTop - e, -120, 120));
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) q[n][i][j] = scaled_half<T>(q[n][i][j], factor);
-                sc[n] = scale2 * __builtin_ldexpf(1.0f, -within(kHalfTop - e, -120, 120));
-            }
-        }
+
         constexpr int KR = sealed ? 2 : 8;
-        u32x4_a kr[KR], kn[KR];                                              // this block's keys, the next one's
-        uint32_t bits = 0, bits_next = 0;
-        // constants of a page: raw, as radii of this lane's 16 pairs, of which page
-        u32x4_a raw_rs[2], raw_rm[2];
+        u32x4_a kr[2][KR], vr[2][8];
+        uint32_t bits[2] = {0, 0};
+        int value_at[2] = {0, 0};
+        uint8_t seen_byte = 0;                // the mask's, of the block that is asked for next
+        u32x4_a raw_rs[2], raw_rm[2];         // constants of the page that is asked for, until its first block's turn
         uint16_t raw_ts = 0, raw_tm = 0;
-        float rs[16], of[16];
+        float rs[16], of[16];                 // radii of this lane's 16 pairs, of the page whose turn it is
         int page_in = -1, page_asked = -1;
-        auto issue = [&](int at, int buf) {
-            const int p = at >> 2, sub = at & 3;
-            const int kp = key_page(c, s, b, p), vp = value_page(c, b, p);
-            const int n = s.kv - at * kTokenBlock;
-            uint32_t seen = n >= 32 ? 0xffffffffu : (1u << n) - 1u;
-            if (a.mask) {
+        auto ask_mask = [&](int at) {
+            if constexpr (MASK) {
                 const int key = at * kTokenBlock + (lane & 31);
-                const bool on = key < s.kv && a.mask[b * a.mask_row + key] != 0;
-                seen &= static_cast<uint32_t>(__ballot(on));
+                seen_byte = a.mask[b * a.mask_row + (key < s.kv ? key : s.kv - 1)];
             }
-            if (kp < 0 || vp < 0) seen = 0;
-            bits_next = __builtin_amdgcn_readfirstlane(seen);
-            if (!bits_next) return;
-            const u32x4_a vb = rows_at(static_cast<const uint16_t*>(c.values.at) + vp * c.values.page + h * c.values.head + sub * (kTokenBlock * 128));
-            const int some = __builtin_ctz(bits_next);                       // rows that are not there are copies of one that is, with weight zero
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int row = 4 * i + (lane >> 4), chunk = r16 ^ ((row & 7) << 1), from = (bits_next >> row) & 1 ? row : some;
-                rows_to_lds(vb, from * 256 + chunk * 16, lds0 + buf * kTokenValues + i * 1024);
+        };
+        auto ask_keys = [&](auto SET, int at) {
+            constexpr int set = decltype(SET)::value;
+            const int p = at >> 2, sub = at & 3;
+            if (p - window >= 64) look_up(p);
+            const int kp = __builtin_amdgcn_readlane(key_ids, p - window), n = s.kv - at * kTokenBlock;
+            value_at[set] = __builtin_amdgcn_readlane(value_ids, p - window);
+            uint32_t there = n >= 32 ? 0xffffffffu : (1u << n) - 1u;
+            if constexpr (MASK) {
+                there &= static_cast<uint32_t>(__ballot(seen_byte != 0));
+                ask_mask(at + 1);
             }
+            bits[set] = kp < 0 ? 0u : there;
             if constexpr (sealed) {
-                const uint8_t* cb = static_cast<const uint8_t*>(c.codes.at) + kp * c.codes.page + h * c.codes.head;
+                const __amdgpu_buffer_rsrc_t from = stream_at(static_cast<const uint8_t*>(c.codes.at) + kp * c.codes.page + h * c.codes.head + sub * kTokenBlock * (PK6 ? 48 : 64),
+                                                              kp < 0 ? 0 : kTokenBlock * (PK6 ? 48 : 64));
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
-                    const int row = sub * kTokenBlock + 16 * u + r16;
                     if constexpr (PK6) {
-                        const uint32_t* w = reinterpret_cast<const uint32_t*>(cb + row * 48 + 12 * g);
-                        kn[u] = u32x4_a{w[0], w[1], w[2], 0u};
+                        typedef uint32_t u32x3_a __attribute__((ext_vector_type(3)));
+                        const u32x3_a w = __builtin_bit_cast(u32x3_a, __builtin_amdgcn_raw_buffer_load_b96(from, r16 * 48 + 12 * g + u * 768, 0, kStream));
+                        kr[set][u] = u32x4_a{w.x, w.y, w.z, 0u};
                     } else {
-                        kn[u] = *reinterpret_cast<const u32x4_a*>(cb + row * 64 + 16 * g);
+                        kr[set][u] = stream16(from, r16 * 64 + 16 * g + u * 1024, 0);
                     }
                 }
-                if (p != page_asked) {
-                    const int64_t at_meta = kp * c.meta.page + h * c.meta.head;
-                    const u32x4_a* prs = reinterpret_cast<const u32x4_a*>(c.rscale + at_meta + 16 * g);
-                    const u32x4_a* prm = reinterpret_cast<const u32x4_a*>(c.rmn + at_meta + 16 * g);
+                if (p != page_asked && kp >= 0) {
+                    page_asked = p;
+                    const int64_t meta = kp * c.meta.page + h * c.meta.head;
+                    const u32x4_a* prs = reinterpret_cast<const u32x4_a*>(c.rscale + meta + 16 * g);
+                    const u32x4_a* prm = reinterpret_cast<const u32x4_a*>(c.rmn + meta + 16 * g);
                     raw_rs[0] = prs[0]; raw_rs[1] = prs[1];
                     raw_rm[0] = prm[0]; raw_rm[1] = prm[1];
-                    raw_ts = c.tscale[at_meta + lane];
-                    raw_tm = c.tmn[at_meta + lane];
-                    page_asked = p;
+                    raw_ts = c.tscale[meta + lane];
+                    raw_tm = c.tmn[meta + lane];
                 }
             } else {
-                const uint16_t* kb = static_cast<const uint16_t*>(c.keys.at) + kp * c.keys.page + h * c.keys.head + sub * (kTokenBlock * 128);
+                const __amdgpu_buffer_rsrc_t from = stream_at(static_cast<const uint16_t*>(c.keys.at) + kp * c.keys.page + h * c.keys.head + sub * (kTokenBlock * 128),
+                                                              kp < 0 ? 0 : kTokenBlock * 256);
 #pragma unroll
                 for (int u = 0; u < 2; u++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        kn[4 * u + i] = *reinterpret_cast<const u32x4_a*>(kb + (16 * u + r16) * 128 + 16 * g + (i >> 1) * 64 + (i & 1) * 8);
+                    for (int i = 0; i < 4; i++) kr[set][4 * u + i] = stream16(from, r16 * 256 + 32 * g + (i >> 1) * 128 + (i & 1) * 16, u * 4096);
+            }
+        };
+        // rows that are not there are zeros: behind the last, or behind the buffer's end where the mask has them
+        auto ask_values = [&](auto SET, int at) {
+            constexpr int set = decltype(SET)::value;
+            const int n = s.kv - at * kTokenBlock;
+            const __amdgpu_buffer_rsrc_t from = stream_at(static_cast<const uint16_t*>(c.values.at) + value_at[set] * c.values.page + h * c.values.head + (at & 3) * (kTokenBlock * 128),
+                                                          bits[set] == 0 ? 0 : n >= 32 ? kTokenBlock * 256 : n * 256);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                uint32_t lane_offset = value_lane + (j & 3) * 256;
+                if constexpr (MASK) lane_offset = (bits[set] >> (4 * g + (j & 3) + 16 * (j >> 2))) & 1 ? lane_offset : 0x10000u;
+                vr[set][j] = stream16(from, lane_offset, (j >> 2) * 4096);
             }
         };
         auto take_page = [&]() {
@@ -236,7 +245,13 @@ __global__ __launch_bounds__(256, 2) void paged_token_kernel(PagedAttnArgs a) {
             for (int k = 0; k < 4; k++) r[k] = __builtin_fmaf(static_cast<float>((r4 >> (8 * k)) & 0xffu), rs[4 * st + k], of[4 * st + k]);
             return quad_of_pairs(r, cs);
         };
-        auto compute = [&](int at, int buf) {
+        auto step = [&](auto SET, int at) {
+            constexpr int set = decltype(SET)::value;
+            const uint32_t there = bits[set];
+            if constexpr (sealed) {
+                const int p = at >> 2;
+                if (page_in != p && page_asked >= p) { take_page(); page_in = p; }       // (before the next page's constants are asked for)
+            }
             floatx4_a z[2][NQ];
 #pragma unroll
             for (int u = 0; u < 2; u++) {
@@ -248,21 +263,22 @@ __global__ __launch_bounds__(256, 2) void paged_token_kernel(PagedAttnArgs a) {
                     if constexpr (sealed) {
                         uint32_t w;
                         if constexpr (PK6) {
-                            const uint32_t d0 = kr[u].x, d1 = kr[u].y, d2 = kr[u].z;
+                            const uint32_t d0 = kr[set][u].x, d1 = kr[set][u].y, d2 = kr[set][u].z;
                             w = unpack_codes6(st == 0 ? d0 : st == 1 ? (d0 >> 24) | (d1 << 8) : st == 2 ? (d1 >> 16) | (d2 << 16) : d2 >> 8);
                         } else {
-                            w = kr[u][st];
+                            w = kr[set][u][st];
                         }
                         kf = key_piece(w, S);
                     } else {
-                        const u32x4_a x = kr[4 * u + (st >> 1)], y = kr[4 * u + 2 + (st >> 1)];
+                        const u32x4_a x = kr[set][4 * u + (st >> 1)], y = kr[set][4 * u + 2 + (st >> 1)];
                         kf = st & 1 ? u32x4_a{x.z, x.w, y.z, y.w} : u32x4_a{x.x, x.y, y.x, y.y};
                     }
 #pragma unroll
                     for (int n = 0; n < NQ; n++) z[u][n] = mma16<TQ>(kf, q[n][st], z[u][n]);
                 });
             }
-            const bool whole = bits == 0xffffffffu && at * kTokenBlock + kTokenBlock - 1 <= first_limit;
+            if (at + 2 < end) ask_keys(SET, at + 2);
+            const bool whole = there == 0xffffffffu && at * kTokenBlock + kTokenBlock - 1 <= first_limit;
             u32x4_a p[NQ];
 #pragma unroll
             for (int n = 0; n < NQ; n++) {
@@ -272,11 +288,11 @@ __global__ __launch_bounds__(256, 2) void paged_token_kernel(PagedAttnArgs a) {
                 for (int e = 0; e < 8; e++) x[e] = z[e >> 2][n][e & 3];
                 if (!whole) {
                     const int last = limit[n] - at * kTokenBlock - 4 * g;
-                    const uint32_t there = bits >> (4 * g);
+                    const uint32_t mine_there = there >> (4 * g);
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
                         const int k = 16 * (e >> 2) + (e & 3);
-                        x[e] = k <= last && (there >> k & 1) ? x[e] : -INFINITY;
+                        x[e] = k <= last && (mine_there >> k & 1) ? x[e] : -INFINITY;
                     }
                 }
                 float mx = x[0];
@@ -300,55 +316,86 @@ __global__ __launch_bounds__(256, 2) void paged_token_kernel(PagedAttnArgs a) {
                 }
                 p[n] = u32x4_a{pack_pair<T>(w[0], w[1]), pack_pair<T>(w[2], w[3]), pack_pair<T>(w[4], w[5]), pack_pair<T>(w[6], w[7])};
             }
+            static_for<4>([&](auto D) {       // channels 8 r16 + 2 d and + 2 d + 1
+                constexpr int d = decltype(D)::value;
+                u32x4_a lo, up;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const u32x2_a w0 = __builtin_bit_cast(u32x2_a, __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_ptr<lds_short4>(tops[i] + buf * kTokenValues)));
-                const u32x2_a w1 = __builtin_bit_cast(u32x2_a, __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_ptr<lds_short4>(tops[i] + buf * kTokenValues + 16 * 256)));
-                const u32x4_a vf = {w0.x, w0.y, w1.x, w1.y};
+                for (int j = 0; j < 4; j++) {
+                    const uint32_t first = vr[set][2 * j][d], second = vr[set][2 * j + 1][d];
+                    lo[j] = __builtin_amdgcn_perm(second, first, 0x05040100u);
+                    up[j] = __builtin_amdgcn_perm(second, first, 0x07060302u);
+                }
 #pragma unroll
-                for (int n = 0; n < NQ; n++) o[n][i] = mma16<T>(vf, p[n], o[n][i]);
-            }
+                for (int n = 0; n < NQ; n++) {
+                    o[n][2 * d] = mma16<T>(lo, p[n], o[n][2 * d]);
+                    o[n][2 * d + 1] = mma16<T>(up, p[n], o[n][2 * d + 1]);
+                }
+            });
+            if (at + 2 < end) ask_values(SET, at + 2);
         };
-        auto arrived = [&]() {
-            rows_arrived();
-            bits = bits_next;
+        ask_mask(blk);
+        ask_keys(IC<0>{}, blk);
+        ask_values(IC<0>{}, blk);
+        if constexpr (sealed) {
+            if (page_asked >= 0) { take_page(); page_in = page_asked; }
+        }
+        if (blk + 1 < end) {
+            ask_keys(IC<1>{}, blk + 1);
+            ask_values(IC<1>{}, blk + 1);
+        }
 #pragma unroll
-            for (int i = 0; i < KR; i++) kr[i] = kn[i];
-        };
-        issue(blk, 0);
-        arrived();
-        for (int buf = 0; blk < end; blk++, buf ^= 1) {
-            if constexpr (sealed) {                                          // (before the next page's constants are asked for)
-                if (bits && page_in != (blk >> 2)) { take_page(); page_in = blk >> 2; }
+        for (int n = 0; n < NQ; n++) {
+            sc[n] = scale2;
+            if constexpr (sealed && std::is_same<T, BF16>::value) {
+                float most = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const uint32_t w = q[n][i][j];
+                        most = fmaxf(most, fmaxf(fabsf(lo2f<T>(static_cast<uint16_t>(w & 0xffffu))), fabsf(lo2f<T>(static_cast<uint16_t>(w >> 16)))));
+                    }
+                most = both_halves_max(both_rows_max(most));
+                const int e = within(kHalfTop - exponent_above(most), -120, 120);
+                const float factor = __builtin_ldexpf(1.0f, e);
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) q[n][i][j] = scaled_half<T>(q[n][i][j], factor);
+                sc[n] = scale2 * __builtin_ldexpf(1.0f, -e);
             }
-            if (blk + 1 < end) issue(blk + 1, buf ^ 1);
-            if (bits) compute(blk, buf);
-            arrived();
+        }
+        for (; blk < end; blk += 2) {
+            step(IC<0>{}, blk);
+            if (blk + 1 < end) step(IC<1>{}, blk + 1);
         }
     };
     walk(std::true_type{}, blk0, blk1 < border ? blk1 : border);
     walk(std::false_type{}, blk0 > border ? blk0 : border, blk1);
 
-    // the four wavefronts' states, joined in the place of their values
-    const uint32_t pairs = lds0 + 2 * kTokenValues;
+    // the four wavefronts' states, joined in LDS
+    __syncthreads();
+    const uint32_t base = lds_addr(sm), states = base + wv * (16 * NQ * 512), pairs = base + 4 * (16 * NQ * 512);
 #pragma unroll
     for (int n = 0; n < NQ; n++) {
         l[n] += __shfl_xor(l[n], 16);
         l[n] += __shfl_xor(l[n], 32);
         const int row = 16 * n + r16;
-        if (g == 0) *lds_ptr<lds_f2>(pairs + row * 8) = floatx2_a{m[n], l[n]};
+        if (g == 0) *lds_ptr<lds_f2>(pairs + (wv * 16 * NQ + row) * 8) = floatx2_a{m[n], l[n]};
 #pragma unroll
-        for (int i = 0; i < 8; i++) *lds_ptr<lds_f4>(lds0 + row * 512 + (((4 * i + g) ^ (row & 15)) * 16)) = float4_v{o[n][i][0], o[n][i][1], o[n][i][2], o[n][i][3]};
+        for (int j = 0; j < 4; j++)           // channels 32 g + 8 j ..
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+                *lds_ptr<lds_f4>(states + row * 512 + ((8 * g + 2 * j + k) ^ r16) * 16) = float4_v{o[n][4 * k][j], o[n][4 * k + 1][j], o[n][4 * k + 2][j], o[n][4 * k + 3][j]};
     }
     __syncthreads();
-    const uint32_t base = lds_addr(sm);
 #pragma unroll
     for (int n = 0; n < NQ; n++) {
         const int row = 16 * n + (tid >> 4), r = row0 + row, ch = tid & 15;              // 16-byte pieces 2 ch and 2 ch + 1 of the row
         float mw[4], lw[4], mx = kNone, sum = 0.0f;
 #pragma unroll
         for (int w = 0; w < 4; w++) {
-            const floatx2_a v = *lds_ptr<lds_f2>(base + w * kTokenWave + 2 * kTokenValues + row * 8);
+            const floatx2_a v = *lds_ptr<lds_f2>(pairs + (w * 16 * NQ + row) * 8);
             mw[w] = v.x; lw[w] = v.y;
             mx = fmaxf(mx, v.x);
         }
@@ -359,7 +406,7 @@ __global__ __launch_bounds__(256, 2) void paged_token_kernel(PagedAttnArgs a) {
             sum = __builtin_fmaf(lw[w], f, sum);
 #pragma unroll
             for (int k = 0; k < 2; k++) {
-                const float4_v v = *lds_ptr<lds_f4>(base + w * kTokenWave + row * 512 + ((2 * ch + k) ^ (row & 15)) * 16);
+                const float4_v v = *lds_ptr<lds_f4>(base + w * (16 * NQ * 512) + row * 512 + ((2 * ch + k) ^ (row & 15)) * 16);
                 acc[4 * k] = __builtin_fmaf(v.x, f, acc[4 * k]); acc[4 * k + 1] = __builtin_fmaf(v.y, f, acc[4 * k + 1]);
                 acc[4 * k + 2] = __builtin_fmaf(v.z, f, acc[4 * k + 2]); acc[4 * k + 3] = __builtin_fmaf(v.w, f, acc[4 * k + 3]);
             }
@@ -422,25 +469,28 @@ int launch_paged_merge(const PagedAttnArgs& a, int dtype, int tile_rows, hipStre
 
 template <typename T, int NQ, bool PK6, bool TABLE>
 static int launch_token(const PagedAttnArgs& a, hipStream_t st) {
-    constexpr int bytes = 4 * kTokenWave;
-    const void* f = reinterpret_cast<const void*>(&paged_token_kernel<T, NQ, PK6, TABLE>);
-    if (const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, bytes); e != hipSuccess) return static_cast<int>(e);
-    const int tiles = (a.max_q * (a.c.N / a.c.Nk) + 16 * NQ - 1) / (16 * NQ);
-    hipLaunchKernelGGL((paged_token_kernel<T, NQ, PK6, TABLE>), dim3(a.c.Nk, tiles * a.n_splits, a.c.B), dim3(256), bytes, st, a);
-    const int err = static_cast<int>(hipGetLastError());
+    auto launch = [&](auto MASK) {
+        constexpr auto kernel = &paged_token_kernel<T, NQ, PK6, TABLE, decltype(MASK)::value>;
+        if constexpr (token_lds<NQ>() > 64 * 1024) {
+            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, token_lds<NQ>());
+            if (e != hipSuccess) return static_cast<int>(e);
+        }
+        const int tiles = (a.max_q * (a.c.N / a.c.Nk) + 16 * NQ - 1) / (16 * NQ);
+        hipLaunchKernelGGL(kernel, dim3(a.c.Nk, tiles * a.n_splits, a.c.B), dim3(256), token_lds<NQ>(), st, a);
+        return static_cast<int>(hipGetLastError());
+    };
+    const int err = a.mask ? launch(std::true_type{}) : launch(std::false_type{});
     return err || a.n_splits == 1 ? err : launch_paged_merge(a, std::is_same<T, F16>::value ? 0 : 1, 16 * NQ, st);
 }
 
-template <typename T, int NQ>
+template <typename T>
 static int launch_token_of(const PagedAttnArgs& a, bool packed, hipStream_t st) {
-    if (packed) return launch_token<T, NQ, true, true>(a, st);
-    return a.c.tbits <= 4 ? launch_token<T, NQ, false, true>(a, st) : launch_token<T, NQ, false, false>(a, st);
+    if (packed) return launch_token<T, 1, true, true>(a, st);
+    return a.c.tbits <= 4 ? launch_token<T, 1, false, true>(a, st) : launch_token<T, 1, false, false>(a, st);
 }
 
 int launch_paged_token(const PagedAttnArgs& a, int dtype, bool packed, hipStream_t st) {
-    const bool few = a.max_q * (a.c.N / a.c.Nk) <= 16;
-    if (dtype == 0) return few ? launch_token_of<F16, 1>(a, packed, st) : launch_token_of<F16, 2>(a, packed, st);
-    return few ? launch_token_of<BF16, 1>(a, packed, st) : launch_token_of<BF16, 2>(a, packed, st);
+    return dtype == 0 ? launch_token_of<F16>(a, packed, st) : launch_token_of<BF16>(a, packed, st);
 }
 
 }  // namespace pq

@@ -182,10 +182,10 @@ PAGED_SIGNATURES = {
     "pq_validate_paged_append": (c_int, _ROWS + [c_void_p] * 4 + [c_void_p] * 5 + [c_int] * 9),
     "pq_paged_append": (c_int, _ROWS + [c_float] + [c_void_p] * 4 + [c_void_p] * 5 + [c_int] * 9 + [c_void_p]),
     "pq_paged_attn_plan": (c_int, [c_int] * 6),
-    "pq_paged_attn_workspace_bytes": (c_size_t, [c_int] * 3),
+    "pq_paged_attn_workspace_bytes": (c_size_t, [c_int] * 5),
     "pq_validate_paged_attn": (c_int, [c_void_p, c_int64] + [c_void_p] * 8 + _TABLES + [c_void_p, c_int64, c_void_p, c_void_p] + [c_int] * 9
                                + [c_void_p, c_size_t, c_int, c_uint]),
-    "pq_paged_attn": (c_int, [c_void_p, c_int64] + [c_void_p] * 8 + _TABLES + [c_void_p, c_int64, c_void_p, c_void_p] + [c_int] * 8 + [c_float, c_int, c_int]
+    "pq_paged_attn": (c_int, [c_void_p, c_int64] + [c_void_p] * 8 + _TABLES + [c_void_p, c_int64, c_void_p, c_void_p] + [c_int] * 8 + [c_float, c_int]
                       + [c_void_p, c_size_t, c_int, c_uint, c_void_p]),
     "pq_validate_paged_weights": (c_int, [c_void_p, c_int64] + [c_void_p] * 8 + _TABLES + [c_void_p, c_int64, c_void_p, c_void_p] + [c_int] * 9 + [c_uint]),
     "pq_paged_weights": (c_int, [c_void_p, c_int64] + [c_void_p] * 8 + _TABLES + [c_void_p, c_int64, c_void_p, c_void_p] + [c_int] * 8 + [c_float, c_int, c_uint, c_void_p]),

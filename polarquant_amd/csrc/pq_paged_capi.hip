@@ -120,19 +120,20 @@ int pq_paged_append(const void* q, int64_t q_row, const void* k, int64_t k_row, 
 }
 
 int pq_paged_attn_plan(int B, int N, int Nk, int max_q, int max_kv, int n_cus) {
-    if (B < 1 || N < 1 || Nk < 1 || N % Nk || max_q < 1 || max_kv < 1) return 1;
-    return pq::paged_splits(B, N, Nk, max_q, max_kv, n_cus);
+    if (B < 1 || N < 1 || Nk < 1 || N % Nk || max_q < 1 || max_kv < 1) return 0;
+    return pq::paged_units(B, N, Nk, max_q, max_kv, n_cus);
 }
 
-size_t pq_paged_attn_workspace_bytes(int T, int N, int n_splits) {
-    if (T < 1 || N < 1 || n_splits <= 1) return 0;
-    return static_cast<size_t>(T) * N * n_splits * (PQ_HEAD_DIM + 2) * sizeof(float);
+size_t pq_paged_attn_workspace_bytes(int B, int N, int Nk, int max_q, int units) {
+    if (B < 1 || N < 1 || Nk < 1 || N % Nk || max_q < 1 || units < 1) return 0;
+    const size_t rows = static_cast<size_t>(units) * Nk * pq::paged_tile_rows(static_cast<int64_t>(max_q) * (N / Nk));
+    return rows * (PQ_HEAD_DIM + 2) * sizeof(float) + static_cast<size_t>(B) * 8;
 }
 
 int pq_validate_paged_attn(const void* q, int64_t q_row, const void* keys, const void* values, const uint8_t* codes, const void* rscale, const void* rmn,
                            const void* tscale, const void* tmn, const int64_t* layout, const int32_t* q_start, const int32_t* kv_len, const int32_t* n_sealed,
                            const int32_t* pages, const int32_t* value_pages, const int32_t* open_pages, int W, int Wo, const uint8_t* mask, int64_t mask_row,
-                           const void* out, const float* lse, int T, int B, int N, int Nk, int max_q, int max_kv, int rbits, int tbits, int n_splits,
+                           const void* out, const float* lse, int T, int B, int N, int Nk, int max_q, int max_kv, int rbits, int tbits, int units,
                            const void* workspace, size_t workspace_bytes, int dtype, unsigned flags) {
     if (!out) return PQ_ERR_NULL_POINTER;
     if (!half_dtype(dtype)) return PQ_ERR_BAD_DTYPE;
@@ -141,12 +142,12 @@ int pq_validate_paged_attn(const void* q, int64_t q_row, const void* keys, const
     if (int rc = check_pages(codes, pages, value_pages, open_pages, Wo, rbits, tbits, flags)) return rc;
     if (int rc = check_queries(q, q_row, N, T)) return rc;
     if (int rc = check_mask(mask, mask_row, B, max_kv)) return rc;
-    const int64_t rows = static_cast<int64_t>(max_q) * (N / Nk), tile = pq::paged_tile_rows(rows);
-    if (n_splits < 1 || (rows + tile - 1) / tile * n_splits > 65535 || (static_cast<int64_t>(max_q) * N + 3) / 4 > INT32_MAX) return PQ_ERR_BAD_SHAPE;
+    const int64_t tiles = pq::paged_tiles(B, N, Nk, max_q);
+    if (units < 0 || units > 65535 || tiles / B > 65535 || static_cast<int64_t>(max_q) * N >= INT32_MAX) return PQ_ERR_BAD_SHAPE;
     if (!aligned(out, 16) || !aligned(lse, 4) || !aligned(workspace, 16)) return PQ_ERR_MISALIGNED;
-    if (n_splits > 1) {
+    if (units > 0) {
         if (!workspace) return PQ_ERR_NULL_POINTER;
-        if (workspace_bytes < pq_paged_attn_workspace_bytes(T, N, n_splits)) return PQ_ERR_WORKSPACE;
+        if (units < tiles || workspace_bytes < pq_paged_attn_workspace_bytes(B, N, Nk, max_q, units)) return PQ_ERR_WORKSPACE;
     }
     return PQ_OK;
 }
@@ -154,10 +155,10 @@ int pq_validate_paged_attn(const void* q, int64_t q_row, const void* keys, const
 int pq_paged_attn(const void* q, int64_t q_row, const void* keys, const void* values, const uint8_t* codes, const void* rscale, const void* rmn,
                   const void* tscale, const void* tmn, const int64_t* layout, const int32_t* q_start, const int32_t* kv_len, const int32_t* n_sealed,
                   const int32_t* pages, const int32_t* value_pages, const int32_t* open_pages, int W, int Wo, const uint8_t* mask, int64_t mask_row, void* out,
-                  float* lse, int T, int B, int N, int Nk, int max_q, int max_kv, int rbits, int tbits, float scale, int n_splits, int n_cus, void* workspace,
+                  float* lse, int T, int B, int N, int Nk, int max_q, int max_kv, int rbits, int tbits, float scale, int units, void* workspace,
                   size_t workspace_bytes, int dtype, unsigned flags, void* stream) {
     if (int rc = pq_validate_paged_attn(q, q_row, keys, values, codes, rscale, rmn, tscale, tmn, layout, q_start, kv_len, n_sealed, pages, value_pages, open_pages,
-                                        W, Wo, mask, mask_row, out, lse, T, B, N, Nk, max_q, max_kv, rbits, tbits, n_splits, workspace, workspace_bytes, dtype, flags))
+                                        W, Wo, mask, mask_row, out, lse, T, B, N, Nk, max_q, max_kv, rbits, tbits, units, workspace, workspace_bytes, dtype, flags))
         return rc;
     pq::PagedAttnArgs a{};
     a.c = cache(keys, values, codes, rscale, rmn, tscale, tmn, layout, q_start, kv_len, n_sealed, pages, value_pages, open_pages, W, Wo, T, B, N, Nk,
@@ -170,8 +171,7 @@ int pq_paged_attn(const void* q, int64_t q_row, const void* keys, const void* va
     a.lse = lse;
     a.partial = static_cast<float*>(workspace);
     a.max_q = max_q;
-    a.n_splits = n_splits;
-    a.slots = 2 * (n_cus > 0 ? n_cus : 256);
+    a.units = units;
     a.scale = scale;
     const bool packed = (flags & PQ_CODES_PACKED6) != 0;
     const hipStream_t st = static_cast<hipStream_t>(stream);

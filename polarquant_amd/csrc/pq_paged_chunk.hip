@@ -1,6 +1,6 @@
 // Attention over the pages of a cache, for many query rows a sequence (a row: a new token and a query head).
 //
-// grid (KV heads, slices x row tiles, sequences), the row tiles that see most first.  Four wavefronts with 32 rows each over 64-key tiles of K and V that
+// grid: paged_unit.  Four wavefronts with 32 rows each over 64-key tiles of K and V that
 // are double-buffered in LDS; all query heads of a KV head share the tiles.  The transposed score tile S^T = K Q^T makes a row a lane, its softmax state a
 // register, and P^T the right operand of O^T = V^T P^T as it stands.
 //
@@ -21,21 +21,18 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttnArgs a) {
     const uint32_t lds0 = uniform(lds_addr(sm));
     const int tid = threadIdx.x, lane = tid & 63, wv = uniform(tid >> 6), col = lane & 31, hi = lane >> 5, i16 = lane & 15, slot = lane >> 4;
     const PagedCache& c = a.c;
-    const int b = blockIdx.z, h = blockIdx.x, slice = blockIdx.y % a.n_splits;
+    PagedUnit unit;
+    if (!paged_unit(c, a.units, kChunkRows, unit)) return;
+    const int b = unit.b, h = blockIdx.x;
     const PagedSequence s = own_sequence(c, b);
-    const int rep = c.N / c.Nk, rows = s.rows * rep, tiles = (rows + kChunkRows - 1) / kChunkRows, tile = tiles - 1 - static_cast<int>(blockIdx.y) / a.n_splits;
-    if (tile < 0) return;
-    const int pages = (s.kv + kPageTokens - 1) / kPageTokens;
-    const int per = pages_per_slice(c, pages, a.n_splits, a.slots, kChunkRows);
-    if (slice > 0 && slice * per >= pages) return;
-    const bool only = per >= pages;
+    const int rep = c.N / c.Nk, rows = s.rows * rep, pages = ceil_div(s.kv, kPageTokens);
 
-    const int row0 = tile * kChunkRows, last_row = row0 + kChunkRows - 1 < rows - 1 ? row0 + kChunkRows - 1 : rows - 1;
+    const int row0 = unit.tile * kChunkRows, last_row = row0 + kChunkRows - 1 < rows - 1 ? row0 + kChunkRows - 1 : rows - 1;
     const int r = row0 + wv * 32 + col, rc = r < rows ? r : rows - 1, token = rc / rep;
     const int limit = s.past + token;                                        // last key this row sees
     const int wave_row = row0 + wv * 32 < rows - 1 ? row0 + wv * 32 : rows - 1, wave_end = wave_row + 31 < rows - 1 ? wave_row + 31 : rows - 1;
     const int wave_first = uniform(s.past + wave_row / rep), wave_last = uniform(s.past + wave_end / rep), last_limit = uniform(s.past + last_row / rep);
-    const int p0 = slice * per, p1 = p0 + per < pages ? p0 + per : pages;
+    const int p0 = min(unit.slice * unit.per, pages), p1 = min(p0 + unit.per, pages);
     const int it0 = 2 * p0;
     int it1 = 2 * p1 < (s.kv + kChunkKeys - 1) / kChunkKeys ? 2 * p1 : (s.kv + kChunkKeys - 1) / kChunkKeys;
     if (const int seen = last_limit < 0 ? 0 : last_limit / kChunkKeys + 1; it1 > seen) it1 = seen;
@@ -100,11 +97,12 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttnArgs a) {
     int raw_key = -1, raw_value = -1;       // of the one behind that
     uint32_t cw[PK6 ? 8 : 4] = {};          // codes of the tile behind the one that is made
     uint2 raw_rs = make_uint2(0, 0), raw_rm = raw_rs, raw_ts = raw_rs, raw_tm = raw_rs;
-    float rs[4] = {}, of[4] = {}, ts[4] = {}, tm[4] = {};
+    uint32_t widths[2] = {}, leasts[2] = {};                                 // of the radii of this lane's four pairs, float16
+    float ts[4] = {}, tm[4] = {};
     float page_scale = 1.0f, page_scale_next = 1.0f;
     uint8_t seen_byte = 1;                  // the mask's, of the tile behind the one that is asked for
     const float angle_bits = 1.0f / static_cast<float>(1 << c.tbits);
-    const uint32_t angles4 = ((1u << c.tbits) - 1u) * 0x01010101u;
+    const uint32_t angles4 = ((1u << c.tbits) - 1u) * 0x01010101u, halves4 = (1u << (c.tbits - 1)) * 0x01010101u;
 
     auto ask_mask = [&](int it) {
         if (!a.mask) return;
@@ -145,24 +143,22 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttnArgs a) {
         float most = 0.0f;
         const float top = static_cast<float>(1 << c.rbits);
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            rs[k] = fourth(raw_rs, k);
-            of[k] = fourth(raw_rm, k);
-            most = fmaxf(most, __builtin_fmaf(fabsf(rs[k]), top, fabsf(of[k])));
-            of[k] = __builtin_fmaf(rs[k], 0.5f, of[k]);
-        }
+        for (int k = 0; k < 4; k++) most = fmaxf(most, __builtin_fmaf(fabsf(fourth(raw_rs, k)), top, fabsf(fourth(raw_rm, k))));
         most = fmaxf(most, __uint_as_float(row_rotate<8>(__float_as_uint(most))));
         most = fmaxf(most, __uint_as_float(row_rotate<4>(__float_as_uint(most))));
         most = fmaxf(most, __uint_as_float(row_rotate<2>(__float_as_uint(most))));
         most = fmaxf(most, __uint_as_float(row_rotate<1>(__float_as_uint(most))));
         const int e = within(kHalfTop - exponent_above(most), -120, 120);
-        const float factor = __builtin_ldexpf(1.0f, e);
+        const float factor = __builtin_ldexpf(1.0f, e), width_factor = factor * angle_bits;
         page_scale_next = __builtin_ldexpf(1.0f, -e);
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            rs[k] *= factor * angle_bits;                                    // (a radius code comes as a byte, above the angle's bits)
-            of[k] *= factor;
-            if constexpr (!TABLE) {
+        for (int k = 0; k < 2; k++) {        // (a radius code comes as a byte, above the angle's bits)
+            widths[k] = pack_pair<F16>(fourth(raw_rs, 2 * k) * width_factor, fourth(raw_rs, 2 * k + 1) * width_factor);
+            leasts[k] = pack_pair<F16>(fourth(raw_rm, 2 * k) * factor, fourth(raw_rm, 2 * k + 1) * factor);
+        }
+        if constexpr (!TABLE) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
                 ts[k] = fourth(raw_ts, k) * kTurn;
                 tm[k] = __builtin_fmaf(ts[k], 0.5f, fourth(raw_tm, k) * kTurn);
             }
@@ -189,7 +185,7 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttnArgs a) {
             else w = cw[j];
             float rad[4];
             uint32_t cs[4];
-            uint32_t r4 = w & ~angles4;
+            uint32_t r4 = (w & ~angles4) | halves4;
             if constexpr (TABLE) {
                 uint32_t a4 = (w & angles4) << 2;
                 asm volatile("" : "+v"(a4), "+v"(r4));
@@ -200,8 +196,7 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttnArgs a) {
 #pragma unroll
                 for (int k = 0; k < 4; k++) cs[k] = cos_sin_half(__builtin_fmaf(static_cast<float>((a4 >> (8 * k)) & 0xffu), ts[k], tm[k]));
             }
-#pragma unroll
-            for (int k = 0; k < 4; k++) rad[k] = __builtin_fmaf(static_cast<float>((r4 >> (8 * k)) & 0xffu), rs[k], of[k]);
+            radii_of(r4, widths[0], widths[1], leasts[0], leasts[1], rad);
             const int row = 16 * wv + 4 * j + slot;
             *lds_ptr<lds_u32x4>(to + row * 256 + (i16 ^ (4 * j + slot)) * 16) = quad_of_pairs(rad, cs);
         }
@@ -392,9 +387,19 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttnArgs a) {
     }
 
     l += __shfl_xor(l, 32);
-    if (r >= rows) return;
-    const size_t at = static_cast<size_t>(s.first + token) * c.N + h * rep + rc % rep;
-    if (only) {
+    if (unit.slices > 1) {
+        const PagedPartials part = paged_partials(a.partial, a.units, c.Nk, kChunkRows);
+        const size_t at = (static_cast<size_t>(blockIdx.y) * c.Nk + h) * kChunkRows + wv * 32 + col;
+        float* out = part.state + at * 128 + 4 * hi;
+        if (r < rows) {
+            static_for<4>([&](auto I) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) *reinterpret_cast<float4*>(out + I * 32 + 8 * j) = make_float4(o[I][4 * j], o[I][4 * j + 1], o[I][4 * j + 2], o[I][4 * j + 3]);
+            });
+            if (hi == 0) part.pair[at] = make_float2(m, l);
+        }
+    } else if (r < rows) {
+        const size_t at = static_cast<size_t>(s.first + token) * c.N + h * rep + rc % rep;
         const float inv = l > 0.0f ? 1.0f / l : 0.0f;
         uint16_t* out = a.out + at * 128 + 4 * hi;
         static_for<4>([&](auto I) {
@@ -403,14 +408,9 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttnArgs a) {
                 *reinterpret_cast<uint2*>(out + I * 32 + 8 * j) = make_uint2(pack_pair<T>(o[I][4 * j] * inv, o[I][4 * j + 1] * inv), pack_pair<T>(o[I][4 * j + 2] * inv, o[I][4 * j + 3] * inv));
         });
         if (a.lse && hi == 0) a.lse[at] = l > 0.0f ? (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f : -INFINITY;
-    } else {
-        float* out = a.partial + (at * a.n_splits + slice) * 128 + 4 * hi;
-        static_for<4>([&](auto I) {
-#pragma unroll
-            for (int j = 0; j < 4; j++) *reinterpret_cast<float4*>(out + I * 32 + 8 * j) = make_float4(o[I][4 * j], o[I][4 * j + 1], o[I][4 * j + 2], o[I][4 * j + 3]);
-        });
-        if (hi == 0) *reinterpret_cast<float2*>(a.partial + static_cast<size_t>(c.T) * c.N * a.n_splits * 128 + 2 * (at * a.n_splits + slice)) = make_float2(m, l);
     }
+    if (a.units && h == 0 && unit.tile == 0 && unit.slice == 0 && tid == 0)
+        paged_partials(a.partial, a.units, c.Nk, kChunkRows).where[b] = make_int2(blockIdx.y, unit.slices);
 }
 
 template <typename T, bool PK6, bool TABLE>
@@ -419,9 +419,9 @@ static int launch_chunk(const PagedAttnArgs& a, hipStream_t st) {
     const void* f = reinterpret_cast<const void*>(&paged_chunk_kernel<T, PK6, TABLE>);
     if (const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, bytes); e != hipSuccess) return static_cast<int>(e);
     const int tiles = (a.max_q * (a.c.N / a.c.Nk) + kChunkRows - 1) / kChunkRows;
-    hipLaunchKernelGGL((paged_chunk_kernel<T, PK6, TABLE>), dim3(a.c.Nk, tiles * a.n_splits, a.c.B), dim3(256), bytes, st, a);
+    hipLaunchKernelGGL((paged_chunk_kernel<T, PK6, TABLE>), a.units ? dim3(a.c.Nk, a.units, 1) : dim3(a.c.Nk, tiles, a.c.B), dim3(256), bytes, st, a);
     const int err = static_cast<int>(hipGetLastError());
-    return err || a.n_splits == 1 ? err : launch_paged_merge(a, std::is_same<T, F16>::value ? 0 : 1, kChunkRows, st);
+    return err || a.units == 0 ? err : launch_paged_merge(a, std::is_same<T, F16>::value ? 0 : 1, kChunkRows, st);
 }
 
 int launch_paged_chunk(const PagedAttnArgs& a, int dtype, bool packed, hipStream_t st) {

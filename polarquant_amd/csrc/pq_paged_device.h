@@ -43,23 +43,100 @@ __device__ __forceinline__ int key_page(const PagedCache& c, const PagedSequence
 }
 __device__ __forceinline__ int value_page(const PagedCache& c, int b, int p) { return page_of(c.value_pages, c.values.n, static_cast<int64_t>(b) * c.W + p); }
 
-// How many pages a slice of the sequence holds.  `slots` workgroups' worth of slices are dealt out over all sequences by their pages and
-// row tiles, so that a batch of unequal sequences keeps the device as busy as an even one; from the device's own lengths, which the host need not know.
-__device__ __forceinline__ int pages_per_slice(const PagedCache& c, int pages, int n_splits, int slots, int tile_rows) {
-    if (n_splits == 1 || pages <= 1) return pages > 0 ? pages : 1;
+// A workgroup's share: a row tile of a sequence and a slice of its pages.
+struct PagedUnit {
+    int b, tile, slice, slices, per;          // per: pages a slice
+};
+
+__device__ __forceinline__ int ceil_div(int v, int d) { return (v + d - 1) / d; }
+__device__ __forceinline__ int wave_total(int v) {
+    v += static_cast<int>(row_rotate<8>(static_cast<uint32_t>(v)));
+    v += static_cast<int>(row_rotate<4>(static_cast<uint32_t>(v)));
+    v += static_cast<int>(row_rotate<2>(static_cast<uint32_t>(v)));
+    v += static_cast<int>(row_rotate<1>(static_cast<uint32_t>(v)));
+    return (__builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 16)) + (__builtin_amdgcn_readlane(v, 32) + __builtin_amdgcn_readlane(v, 48));
+}
+
+// Not cut (units 0): grid (.., row tiles of the longest call, sequences), the last tiles, which see most, first.  Otherwise `units` workgroups a KV head are dealt out over the
+// sequences' pages, by the lengths that the device finds: slices as long as makes their number fit, so that all stand on the device at once whatever the lengths are.
+// Every wavefront comes to the same result by itself, a lane a sequence.  false: nothing is left for this workgroup.
+__device__ __forceinline__ bool paged_unit(const PagedCache& c, int units, int tile_rows, PagedUnit& u) {
     const int rep = c.N / c.Nk;
-    int64_t total = 0;
-    for (int i = threadIdx.x & 63; i < c.B; i += kWave) {
-        const PagedSequence s = paged_sequence(c, i);
-        total += static_cast<int64_t>((s.kv + kPageTokens - 1) / kPageTokens) * ((s.rows * rep + tile_rows - 1) / tile_rows);
+    if (units == 0) {
+        const PagedSequence s = own_sequence(c, blockIdx.z);
+        const int pages = ceil_div(s.kv, kPageTokens);
+        u.b = blockIdx.z;
+        u.tile = ceil_div(s.rows * rep, tile_rows) - 1 - static_cast<int>(blockIdx.y);
+        u.slice = 0;
+        u.slices = 1;
+        u.per = pages > 0 ? pages : 1;
+        return u.tile >= 0;
     }
+    const int lane = threadIdx.x & 63, id = blockIdx.y;
+    int pages = 0, tiles = 0;
+    auto extent = [&](int b) {
+        const PagedSequence s = paged_sequence(c, b < c.B ? b : c.B - 1);
+        pages = ceil_div(s.kv, kPageTokens);
+        pages = pages > 0 ? pages : 1;
+        tiles = b < c.B ? ceil_div(s.rows * rep, tile_rows) : 0;
+    };
+    extent(lane);
+    // (far more than there are units is as good as too many)
+    auto slices_of = [&](int per) { return static_cast<int>(fminf(static_cast<float>(tiles) * static_cast<float>(ceil_div(pages, per)), 1e6f)); };
+    int per = 0, all = 0, most = 1;
+    for (int b = lane; b - lane < c.B; b += kWave) {
+        if (c.B > kWave) extent(b);
+        all += wave_total(slices_of(1));
+    }
+    per = max(1, ceil_div(all, units));
+    for (int k = 0; k < 16; k++) {            // (a share may end inside: longer slices until their number fits)
+        int count = 0;
+        most = 0;
+        for (int b = lane; b - lane < c.B; b += kWave) {
+            if (c.B > kWave) extent(b);
+            count += wave_total(slices_of(per));
+            most += wave_total(tiles && pages > per ? 1 : 0);
+        }
+        if (count <= units) break;
+        if (k == 15 || most == 0) { per = 1 << 24; break; }                  // (as many units as row tiles at least: uncut they fit)
+        per = max(per + 1, static_cast<int>(static_cast<float>(per) * static_cast<float>(count) / static_cast<float>(units)));
+    }
+    int before = 0;
+    for (int b = lane; b - lane < c.B; b += kWave) {
+        if (c.B > kWave) extent(b);
+        const int n = slices_of(per);
+        int end = n;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o);
-    int64_t per = (total * c.Nk + slots - 1) / slots;
-    per = per < 1 ? 1 : per > pages ? pages : per;
-    int n = (pages + static_cast<int>(per) - 1) / static_cast<int>(per);
-    n = n < n_splits ? n : n_splits;
-    return uniform((pages + n - 1) / n);
+        for (int o = 1; o < kWave; o <<= 1) {
+            const int v = __shfl_up(end, o);
+            end += lane >= o ? v : 0;
+        }
+        const uint64_t here = __ballot(before + end > id);
+        if (here) {
+            const int at = __builtin_ctzll(here);
+            const int slices = ceil_div(__builtin_amdgcn_readlane(pages, at), per), k = id - before - (__builtin_amdgcn_readlane(end, at) - __builtin_amdgcn_readlane(n, at));
+            u.b = b - lane + at;
+            u.tile = k / slices;
+            u.slice = k % slices;
+            u.slices = slices;
+            u.per = ceil_div(__builtin_amdgcn_readlane(pages, at), slices);
+            return true;
+        }
+        before += __builtin_amdgcn_readlane(end, 63);
+    }
+    return false;
+}
+
+// Where the slices' states are kept until they are joined: of unit i and KV head h, [rows of a tile, 128] floats, [rows of a tile] pairs (maximum in log2 units, sum), and of
+// every sequence the unit of its first slice and the slices of a row tile.
+struct PagedPartials {
+    float* state;
+    float2* pair;
+    int2* where;
+};
+__device__ __forceinline__ PagedPartials paged_partials(float* at, int units, int Nk, int tile_rows) {
+    const size_t rows = static_cast<size_t>(units) * Nk * tile_rows;
+    return PagedPartials{at, reinterpret_cast<float2*>(at + rows * 128), reinterpret_cast<int2*>(at + rows * 130)};
 }
 
 __device__ __forceinline__ float both_rows_max(float v) {        // of lanes l and l ^ 16
@@ -108,6 +185,24 @@ __device__ __forceinline__ void times_half(uint32_t& w, float r, uint32_t cs) {
     else if constexpr (LO) asm("v_fma_mixlo_f16 %0, %1, %2, 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]" : "=v"(w) : "v"(r), "v"(cs));
     else if constexpr (!SIN) asm("v_fma_mixhi_f16 %0, %1, %2, 0 op_sel_hi:[0,1,0]" : "+v"(w) : "v"(r), "v"(cs));
     else asm("v_fma_mixhi_f16 %0, %1, %2, 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]" : "+v"(w) : "v"(r), "v"(cs));
+}
+
+// a * (a half of b) + (the same half of c)
+template <bool HIGH>
+__device__ __forceinline__ float times_plus_half(float a, uint32_t b, uint32_t c) {
+    float r;
+    if constexpr (HIGH) asm("v_fma_mix_f32 %0, %1, %2, %3 op_sel:[0,1,1] op_sel_hi:[0,1,1]" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    else asm("v_fma_mix_f32 %0, %1, %2, %3 op_sel_hi:[0,1,1]" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
+// Radii of four pairs from a word of codes whose angles' bits are gone and have the lowest radius bit's half in their place: each byte is (rho + 1/2)
+// 2^tbits, exactly.  widths, leasts: float16, two words each.
+__device__ __forceinline__ void radii_of(uint32_t r4, uint32_t w0, uint32_t w1, uint32_t l0, uint32_t l1, float (&r)[4]) {
+    r[0] = times_plus_half<false>(static_cast<float>(r4 & 0xffu), w0, l0);
+    r[1] = times_plus_half<true>(static_cast<float>((r4 >> 8) & 0xffu), w0, l0);
+    r[2] = times_plus_half<false>(static_cast<float>((r4 >> 16) & 0xffu), w1, l1);
+    r[3] = times_plus_half<true>(static_cast<float>(r4 >> 24), w1, l1);
 }
 
 // 16 bytes of a key: pairs 4 c .. 4 c + 3 as (x x x x y y y y), from their radii and angles' cos and sin

@@ -32,8 +32,8 @@ struct PagedAttnArgs {
     int64_t mask_row;
     uint16_t* out;                            // [T, N, 128]
     float* lse;                               // [T, N] or null
-    float* partial;                           // [T * N, n_splits, 128], then [T * N, n_splits] pairs (maximum in log2 units, sum)
-    int max_q, n_splits, slots;               // slices a sequence is cut into at most; workgroups that the device holds
+    float* partial;                           // the slices' states (PagedPartials)
+    int max_q, units;                         // workgroups a KV head that the pages are dealt out to; 0: a sequence is not cut
     float scale;
 };
 int launch_paged_token(const PagedAttnArgs& a, int dtype, bool packed, hipStream_t st);

@@ -1,6 +1,6 @@
 // Attention over the pages of a cache, for few query rows a sequence (a row: a new token and a query head), and the merge of its slices.
 //
-// grid (KV heads, slices x row tiles, sequences).  A workgroup owns 16 NQ rows and a slice of whole pages; its four wavefronts divide the slice's
+// grid: paged_unit.  A workgroup owns 16 NQ rows and a slice of whole pages; its four wavefronts divide the slice's
 // blocks of 32 tokens among them and run on their own until their states are joined in LDS, so nothing waits at a barrier.  The score tile is transposed, S^T = K
 // Q^T: a row is a lane, its softmax state a register, and the weights are the right operand of O^T = V^T P^T as they stand.
 //
@@ -11,7 +11,7 @@
 //
 // Angles go through a table of cos and sin in LDS, 64 pairs x 16 bins of float16, which a wavefront makes once a page: word (pair % 16) 64 +
 // (pair / 16) 16 + bin, so that the lanes of a lookup, four pairs and sixteen keys, meet a bank only with a lane that wants the same word.
-// (More than 16 bins: cos and sin are evaluated for every code.)  Radii are (code) x (width of a bin) + (least and half a width).
+// (More than 16 bins: cos and sin are evaluated for every code.)  Radii are (code + 1/2) (width of a bin) + (least).
 #include "pq_paged_device.h"
 
 namespace pq {
@@ -33,15 +33,14 @@ template <typename T, int NQ, bool PK6, bool TABLE, bool MASK>
 __global__ __launch_bounds__(256, 2) void paged_token_kernel(PagedAttnArgs a) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t sm[];
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, g = lane >> 4;
-    const int b = blockIdx.z, h = blockIdx.x, slice = blockIdx.y % a.n_splits, tile = blockIdx.y / a.n_splits;
+    const int h = blockIdx.x;
     const PagedCache& c = a.c;
+    PagedUnit unit;
+    if (!paged_unit(c, a.units, 16 * NQ, unit)) return;
+    const int b = unit.b;
     const PagedSequence s = own_sequence(c, b);
-    const int rep = c.N / c.Nk, rows = s.rows * rep, row0 = tile * 16 * NQ;
-    if (row0 >= rows) return;
-    const int pages = (s.kv + kPageTokens - 1) / kPageTokens;
-    const int per = pages_per_slice(c, pages, a.n_splits, a.slots, 16 * NQ);
-    if (slice > 0 && slice * per >= pages) return;
-    const bool only = per >= pages;
+    const int rep = c.N / c.Nk, rows = s.rows * rep, row0 = unit.tile * 16 * NQ, pages = ceil_div(s.kv, kPageTokens);
+    const bool only = unit.slices == 1;
     const uint32_t table = uniform(lds_addr(sm) + wv * kTokenTable);
 
     // this lane's rows, the keys they see, and their queries: 16 channels from 16 g on and 16 from 64 + 16 g on, which is the order of a key's pairs
@@ -75,7 +74,7 @@ __global__ __launch_bounds__(256, 2) void paged_token_kernel(PagedAttnArgs a) {
 
     // this wavefront's blocks
     int blocks = (s.kv + kTokenBlock - 1) / kTokenBlock;
-    const int p0 = slice * per, p1 = p0 + per < pages ? p0 + per : pages;
+    const int p0 = min(unit.slice * unit.per, pages), p1 = min(p0 + unit.per, pages);
     const int mine = p1 - p0;                 // (a quarter of four blocks a page)
     const int blk0 = 4 * p0 + wv * mine;
     const int seen = last_limit < 0 ? 0 : last_limit / kTokenBlock + 1;
@@ -93,7 +92,7 @@ __global__ __launch_bounds__(256, 2) void paged_token_kernel(PagedAttnArgs a) {
         for (int i = 0; i < 8; i++) o[n][i] = floatx4_a{0.0f, 0.0f, 0.0f, 0.0f};
     }
     const float rest = 1.0f / static_cast<float>(1 << c.tbits);
-    const uint32_t angles4 = ((1u << c.tbits) - 1u) * 0x01010101u;
+    const uint32_t angles4 = ((1u << c.tbits) - 1u) * 0x01010101u, halves4 = (1u << (c.tbits - 1)) * 0x01010101u;
     const uint32_t value_lane = g * 1024 + r16 * 16;                         // tokens 4 g + j and 16 + 4 g + j, channels 8 r16 ..
 
     auto walk = [&](auto SEALED, int blk, const int end) {
@@ -124,7 +123,7 @@ __global__ __launch_bounds__(256, 2) void paged_token_kernel(PagedAttnArgs a) {
         uint8_t seen_byte = 0;                // the mask's, of the block that is asked for next
         u32x4_a raw_rs[2], raw_rm[2];         // constants of the page that is asked for, until its first block's turn
         uint16_t raw_ts = 0, raw_tm = 0;
-        float rs[16], of[16];                 // radii of this lane's 16 pairs, of the page whose turn it is
+        uint32_t widths[8], leasts[8];        // of the radii of this lane's 16 pairs, float16, of the page whose turn it is
         int page_in = -1, page_asked = -1;
         auto ask_mask = [&](int at) {
             if constexpr (MASK) {
@@ -132,11 +131,12 @@ __global__ __launch_bounds__(256, 2) void paged_token_kernel(PagedAttnArgs a) {
                 seen_byte = a.mask[b * a.mask_row + (key < s.kv ? key : s.kv - 1)];
             }
         };
-        auto ask_keys = [&](auto SET, int at) {
+        // (Asked for in any case, behind the end nothing: the compiler counts loads in flight, and where paths meet the fewest.)
+        auto ask_keys = [&](auto SET, int asked) {
             constexpr int set = decltype(SET)::value;
-            const int p = at >> 2, sub = at & 3;
+            const int at = asked < end ? asked : end - 1, p = at >> 2, sub = at & 3;
             if (p - window >= 64) look_up(p);
-            const int kp = __builtin_amdgcn_readlane(key_ids, p - window), n = s.kv - at * kTokenBlock;
+            const int id = __builtin_amdgcn_readlane(key_ids, p - window), kp = asked < end ? id : -1, n = s.kv - at * kTokenBlock;
             value_at[set] = __builtin_amdgcn_readlane(value_ids, p - window);
             uint32_t there = n >= 32 ? 0xffffffffu : (1u << n) - 1u;
             if constexpr (MASK) {
@@ -160,12 +160,11 @@ __global__ __launch_bounds__(256, 2) void paged_token_kernel(PagedAttnArgs a) {
                 if (p != page_asked && kp >= 0) {
                     page_asked = p;
                     const int64_t meta = kp * c.meta.page + h * c.meta.head;
-                    const u32x4_a* prs = reinterpret_cast<const u32x4_a*>(c.rscale + meta + 16 * g);
-                    const u32x4_a* prm = reinterpret_cast<const u32x4_a*>(c.rmn + meta + 16 * g);
-                    raw_rs[0] = prs[0]; raw_rs[1] = prs[1];
-                    raw_rm[0] = prm[0]; raw_rm[1] = prm[1];
-                    raw_ts = c.tscale[meta + lane];
-                    raw_tm = c.tmn[meta + lane];
+                    const __amdgpu_buffer_rsrc_t ws = stream_at(c.rscale + meta, 128), wm = stream_at(c.rmn + meta, 128);
+                    raw_rs[0] = stream16(ws, 32 * g, 0); raw_rs[1] = stream16(ws, 32 * g + 16, 0);
+                    raw_rm[0] = stream16(wm, 32 * g, 0); raw_rm[1] = stream16(wm, 32 * g + 16, 0);
+                    raw_ts = __builtin_amdgcn_raw_buffer_load_b16(stream_at(c.tscale + meta, 128), 2 * lane, 0, 0);
+                    raw_tm = __builtin_amdgcn_raw_buffer_load_b16(stream_at(c.tmn + meta, 128), 2 * lane, 0, 0);
                 }
             } else {
                 const __amdgpu_buffer_rsrc_t from = stream_at(static_cast<const uint16_t*>(c.keys.at) + kp * c.keys.page + h * c.keys.head + sub * (kTokenBlock * 128),
@@ -177,8 +176,9 @@ __global__ __launch_bounds__(256, 2) void paged_token_kernel(PagedAttnArgs a) {
             }
         };
         // rows that are not there are zeros: behind the last, or behind the buffer's end where the mask has them
-        auto ask_values = [&](auto SET, int at) {
+        auto ask_values = [&](auto SET, int asked) {
             constexpr int set = decltype(SET)::value;
+            const int at = asked < end ? asked : end - 1;
             const int n = s.kv - at * kTokenBlock;
             const __amdgpu_buffer_rsrc_t from = stream_at(static_cast<const uint16_t*>(c.values.at) + value_at[set] * c.values.page + h * c.values.head + (at & 3) * (kTokenBlock * 128),
                                                           bits[set] == 0 ? 0 : n >= 32 ? kTokenBlock * 256 : n * 256);
@@ -192,22 +192,20 @@ __global__ __launch_bounds__(256, 2) void paged_token_kernel(PagedAttnArgs a) {
         auto take_page = [&]() {
             float most = 0.0f;
             const float top = static_cast<float>(1 << c.rbits);
+            auto half = [](uint32_t w, int k) { return lo2f<T>(static_cast<uint16_t>(k ? w >> 16 : w & 0xffffu)); };
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const uint32_t ws = raw_rs[i >> 3][(i & 7) >> 1], wm = raw_rm[i >> 3][(i & 7) >> 1];
-                rs[i] = lo2f<T>(static_cast<uint16_t>(i & 1 ? ws >> 16 : ws & 0xffffu));
-                of[i] = lo2f<T>(static_cast<uint16_t>(i & 1 ? wm >> 16 : wm & 0xffffu));
-                most = fmaxf(most, __builtin_fmaf(fabsf(rs[i]), top, fabsf(of[i])));
-                of[i] = __builtin_fmaf(rs[i], 0.5f, of[i]);
-            }
+            for (int i = 0; i < 8; i++)
+#pragma unroll
+                for (int k = 0; k < 2; k++) most = fmaxf(most, __builtin_fmaf(fabsf(half(raw_rs[i >> 2][i & 3], k)), top, fabsf(half(raw_rm[i >> 2][i & 3], k))));
             most = both_halves_max(both_rows_max(most));
             const int e = within(kHalfTop - exponent_above(most), -120, 120);
-            const float factor = __builtin_ldexpf(1.0f, e);
+            const float factor = __builtin_ldexpf(1.0f, e), width_factor = factor * rest;
             page_scale = __builtin_ldexpf(1.0f, -e);
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                rs[i] *= factor * rest;                                      // (a radius code comes as a byte, above the angle's bits)
-                of[i] *= factor;
+            for (int i = 0; i < 8; i++) {     // (a radius code comes as a byte, above the angle's bits)
+                const uint32_t ws = raw_rs[i >> 2][i & 3], wm = raw_rm[i >> 2][i & 3];
+                widths[i] = pack_pair<F16>(half(ws, 0) * width_factor, half(ws, 1) * width_factor);
+                leasts[i] = pack_pair<F16>(half(wm, 0) * factor, half(wm, 1) * factor);
             }
             const float ts = lo2f<T>(raw_ts) * kTurn, tm = __builtin_fmaf(ts, 0.5f, lo2f<T>(raw_tm) * kTurn);
             if constexpr (TABLE) {
@@ -227,7 +225,7 @@ __global__ __launch_bounds__(256, 2) void paged_token_kernel(PagedAttnArgs a) {
             constexpr int st = decltype(S)::value;
             float r[4];
             uint32_t cs[4];
-            uint32_t r4 = w & ~angles4;
+            uint32_t r4 = (w & ~angles4) | halves4;
             if constexpr (TABLE) {
                 uint32_t a4 = (w & angles4) << 2;
                 asm volatile("" : "+v"(a4), "+v"(r4));
@@ -241,8 +239,7 @@ __global__ __launch_bounds__(256, 2) void paged_token_kernel(PagedAttnArgs a) {
                     cs[k] = cos_sin_half(__builtin_fmaf(static_cast<float>((a4 >> (8 * k)) & 0xffu), t.x, t.y));
                 }
             }
-#pragma unroll
-            for (int k = 0; k < 4; k++) r[k] = __builtin_fmaf(static_cast<float>((r4 >> (8 * k)) & 0xffu), rs[4 * st + k], of[4 * st + k]);
+            radii_of(r4, widths[2 * st], widths[2 * st + 1], leasts[2 * st], leasts[2 * st + 1], r);
             return quad_of_pairs(r, cs);
         };
         auto step = [&](auto SET, int at) {
@@ -277,7 +274,7 @@ __global__ __launch_bounds__(256, 2) void paged_token_kernel(PagedAttnArgs a) {
                     for (int n = 0; n < NQ; n++) z[u][n] = mma16<TQ>(kf, q[n][st], z[u][n]);
                 });
             }
-            if (at + 2 < end) ask_keys(SET, at + 2);
+            ask_keys(SET, at + 2);
             const bool whole = there == 0xffffffffu && at * kTokenBlock + kTokenBlock - 1 <= first_limit;
             u32x4_a p[NQ];
 #pragma unroll
@@ -331,7 +328,7 @@ __global__ __launch_bounds__(256, 2) void paged_token_kernel(PagedAttnArgs a) {
                     o[n][2 * d + 1] = mma16<T>(up, p[n], o[n][2 * d + 1]);
                 }
             });
-            if (at + 2 < end) ask_values(SET, at + 2);
+            ask_values(SET, at + 2);
         };
         ask_mask(blk);
         ask_keys(IC<0>{}, blk);
@@ -339,10 +336,8 @@ __global__ __launch_bounds__(256, 2) void paged_token_kernel(PagedAttnArgs a) {
         if constexpr (sealed) {
             if (page_asked >= 0) { take_page(); page_in = page_asked; }
         }
-        if (blk + 1 < end) {
-            ask_keys(IC<1>{}, blk + 1);
-            ask_values(IC<1>{}, blk + 1);
-        }
+        ask_keys(IC<1>{}, blk + 1);
+        ask_values(IC<1>{}, blk + 1);
 #pragma unroll
         for (int n = 0; n < NQ; n++) {
             sc[n] = scale2;
@@ -365,10 +360,11 @@ __global__ __launch_bounds__(256, 2) void paged_token_kernel(PagedAttnArgs a) {
                 sc[n] = scale2 * __builtin_ldexpf(1.0f, -e);
             }
         }
-        for (; blk < end; blk += 2) {
+        for (; blk + 1 < end; blk += 2) {
             step(IC<0>{}, blk);
-            if (blk + 1 < end) step(IC<1>{}, blk + 1);
+            step(IC<1>{}, blk + 1);
         }
+        if (blk < end) step(IC<0>{}, blk);
     };
     walk(std::true_type{}, blk0, blk1 < border ? blk1 : border);
     walk(std::false_type{}, blk0 > border ? blk0 : border, blk1);
@@ -411,50 +407,52 @@ __global__ __launch_bounds__(256, 2) void paged_token_kernel(PagedAttnArgs a) {
                 acc[4 * k + 2] = __builtin_fmaf(v.z, f, acc[4 * k + 2]); acc[4 * k + 3] = __builtin_fmaf(v.w, f, acc[4 * k + 3]);
             }
         }
-        if (r >= rows) continue;
-        const size_t at = static_cast<size_t>(s.first + r / rep) * c.N + h * rep + r % rep;
-        if (only) {
-            const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-            *reinterpret_cast<uint4*>(a.out + at * 128 + 8 * ch) = make_uint4(pack_pair<T>(acc[0] * inv, acc[1] * inv), pack_pair<T>(acc[2] * inv, acc[3] * inv),
-                                                                              pack_pair<T>(acc[4] * inv, acc[5] * inv), pack_pair<T>(acc[6] * inv, acc[7] * inv));
-            if (a.lse && ch == 0) a.lse[at] = sum > 0.0f ? (mx + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f : -INFINITY;
-        } else {
-            float* to = a.partial + (at * a.n_splits + slice) * 128 + 8 * ch;
+        if (!only) {
+            const PagedPartials part = paged_partials(a.partial, a.units, c.Nk, 16 * NQ);
+            const size_t at = (static_cast<size_t>(blockIdx.y) * c.Nk + h) * (16 * NQ) + row;
+            float* to = part.state + at * 128 + 8 * ch;
             *reinterpret_cast<float4*>(to) = make_float4(acc[0], acc[1], acc[2], acc[3]);
             *reinterpret_cast<float4*>(to + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
-            if (ch == 0) *reinterpret_cast<float2*>(a.partial + static_cast<size_t>(c.T) * c.N * a.n_splits * 128 + 2 * (at * a.n_splits + slice)) = make_float2(mx, sum);
+            if (ch == 0) part.pair[at] = make_float2(mx, sum);
+            continue;
         }
+        if (r >= rows) continue;
+        const size_t at = static_cast<size_t>(s.first + r / rep) * c.N + h * rep + r % rep;
+        const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+        *reinterpret_cast<uint4*>(a.out + at * 128 + 8 * ch) = make_uint4(pack_pair<T>(acc[0] * inv, acc[1] * inv), pack_pair<T>(acc[2] * inv, acc[3] * inv),
+                                                                          pack_pair<T>(acc[4] * inv, acc[5] * inv), pack_pair<T>(acc[6] * inv, acc[7] * inv));
+        if (a.lse && ch == 0) a.lse[at] = sum > 0.0f ? (mx + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f : -INFINITY;
     }
+    if (a.units && h == 0 && unit.tile == 0 && unit.slice == 0 && tid == 0)
+        paged_partials(a.partial, a.units, c.Nk, 16 * NQ).where[b] = make_int2(blockIdx.y, unit.slices);
 }
 
-// One wavefront joins a row's slices: lane i the weight of slices i, i + 64, .., then two channels.
+// One wavefront joins a row's slices: lane i the weight of slice i, then two channels.
 template <typename T>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a, int tile_rows) {
     const PagedCache& c = a.c;
-    const int b = blockIdx.y, lane = threadIdx.x & 63;
-    const PagedSequence s = own_sequence(c, b);
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    if (i >= static_cast<int64_t>(s.rows) * c.N) return;
-    const int pages = (s.kv + kPageTokens - 1) / kPageTokens;
-    const int per = pages_per_slice(c, pages, a.n_splits, a.slots, tile_rows);
-    if (per >= pages) return;                                                // (written by its only slice)
-    const int n = (pages + per - 1) / per;
-    const size_t at = static_cast<size_t>(s.first) * c.N + i;
-    const float2* ml = reinterpret_cast<const float2*>(a.partial + static_cast<size_t>(c.T) * c.N * a.n_splits * 128) + at * a.n_splits;
+    const int b = blockIdx.y, lane = threadIdx.x & 63, rep = c.N / c.Nk;
+    const PagedPartials part = paged_partials(a.partial, a.units, c.Nk, tile_rows);
+    const int2 where = part.where[b];
+    const int first = within(c.q_start[b], 0, c.T), tokens = within(c.q_start[b + 1], first, c.T) - first;
+    const int i = static_cast<int>(blockIdx.x) * 4 + uniform(static_cast<int>(threadIdx.x >> 6)), token = i / c.N, head = i % c.N;
+    if (token >= tokens || where.y <= 1) return;                             // (of one slice: written by it)
+    const int h = head / rep, r = token * rep + head % rep, unit = where.x + r / tile_rows * where.y;
+    const size_t row = (static_cast<size_t>(unit) * c.Nk + h) * tile_rows + r % tile_rows, step = static_cast<size_t>(c.Nk) * tile_rows;
     float mx = kNone;
-    for (int j = lane; j < n; j += kWave) mx = fmaxf(mx, ml[j].x);
+    for (int j = lane; j < where.y; j += kWave) mx = fmaxf(mx, part.pair[row + j * step].x);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-    const float* part = a.partial + at * a.n_splits * 128 + 2 * lane;
     float sum = 0.0f, x = 0.0f, y = 0.0f;
 #pragma unroll 8
-    for (int j = 0; j < n; j++) {
-        const float2 v = ml[j], p = *reinterpret_cast<const float2*>(part + j * 128);
+    for (int j = 0; j < where.y; j++) {
+        const float2 v = part.pair[row + j * step], p = *reinterpret_cast<const float2*>(part.state + (row + j * step) * 128 + 2 * lane);
         const float f = exp2_hw(v.x - mx);
         sum = __builtin_fmaf(v.y, f, sum);
         x = __builtin_fmaf(p.x, f, x);
         y = __builtin_fmaf(p.y, f, y);
     }
+    const size_t at = static_cast<size_t>(first + token) * c.N + head;
     const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
     *reinterpret_cast<uint32_t*>(a.out + at * 128 + 2 * lane) = pack_pair<T>(x * inv, y * inv);
     if (a.lse && lane == 0) a.lse[at] = sum > 0.0f ? (mx + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f : -INFINITY;
@@ -476,11 +474,11 @@ static int launch_token(const PagedAttnArgs& a, hipStream_t st) {
             if (e != hipSuccess) return static_cast<int>(e);
         }
         const int tiles = (a.max_q * (a.c.N / a.c.Nk) + 16 * NQ - 1) / (16 * NQ);
-        hipLaunchKernelGGL(kernel, dim3(a.c.Nk, tiles * a.n_splits, a.c.B), dim3(256), token_lds<NQ>(), st, a);
+        hipLaunchKernelGGL(kernel, a.units ? dim3(a.c.Nk, a.units, 1) : dim3(a.c.Nk, tiles, a.c.B), dim3(256), token_lds<NQ>(), st, a);
         return static_cast<int>(hipGetLastError());
     };
     const int err = a.mask ? launch(std::true_type{}) : launch(std::false_type{});
-    return err || a.n_splits == 1 ? err : launch_paged_merge(a, std::is_same<T, F16>::value ? 0 : 1, 16 * NQ, st);
+    return err || a.units == 0 ? err : launch_paged_merge(a, std::is_same<T, F16>::value ? 0 : 1, 16 * NQ, st);
 }
 
 template <typename T>

@@ -165,20 +165,21 @@ def seal_pages(pool: PagePool, batch: PageBatch, eager_gpu: bool = False) -> Non
 
 
 def paged_attention(q: torch.Tensor, pool: PagePool, batch: PageBatch, attention_mask: Optional[torch.Tensor] = None, sm_scale: Optional[float] = None,
-                    return_lse: bool = False, n_splits: Optional[int] = None, workspace: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None):
+                    return_lse: bool = False, units: Optional[int] = None, workspace: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None):
     """q [T, N, 128] (rotated queries of the new tokens, packed) -> [T, N, 128]: each attends to its sequence's keys up to its own.  attention_mask [B, >=
     max_kv] of {0, 1}: keys that are not there.  A row without a key is zero.  return_lse: also float32 [T, N], the natural logarithm of each row's sum of
-    exponentials (for `page_weights`).  The context is cut into up to `n_splits` slices through `workspace` (float32, of
-    paged_workspace_bytes(T, N, n_splits); by default memory of this call alone, so calls of several streams and graphs do not meet)."""
+    exponentials (for `page_weights`).  The pages are dealt out to `units` workgroups a KV head (0: no
+    sequence is cut) through `workspace` (float32, of paged_workspace_bytes(batch, N, Nk, units); by default memory of this call alone, so calls of several streams and
+    graphs do not meet)."""
     _gpu(q)
     _same(pool, batch, q, attention_mask, workspace, out)
     q, q_row, T, N = _heads(q, "q")
     _refuse(q.dtype != pool.dtype or N % pool.n_kv_heads != 0, "q must be %s, with a multiple of %d heads", pool.dtype, pool.n_kv_heads)
     mask, mask_row = _mask(attention_mask, batch)
     lib, max_q, cus = _ffi.paged_lib().call, min(batch.max_q, T), _num_cus(pool.device)
-    if n_splits is None:
-        n_splits = lib.pq_paged_attn_plan(batch.size, N, pool.n_kv_heads, max_q, batch.max_kv, cus)
-    need = lib.pq_paged_attn_workspace_bytes(T, N, n_splits)
+    if units is None:
+        units = lib.pq_paged_attn_plan(batch.size, N, pool.n_kv_heads, max_q, batch.max_kv, cus)
+    need = lib.pq_paged_attn_workspace_bytes(batch.size, N, pool.n_kv_heads, max_q, units) if units else 0
     if workspace is None:
         workspace = _calls.empty(q, 3, need // 4) if need else None
     else:
@@ -190,14 +191,14 @@ def paged_attention(q: torch.Tensor, pool: PagePool, batch: PageBatch, attention
     with _on_device(pool.device):
         rc = lib.pq_paged_attn(q, q_row, pool.keys, pool.values, pool.codes, *pool.meta, pool.layout, batch.q_start, batch.kv_len, batch.n_sealed, batch.pages,
                                batch.value_pages, batch.open_pages, batch.width, batch.open_width, mask, mask_row, out, lse, T, batch.size, N, pool.n_kv_heads,
-                               max_q, batch.max_kv, pool.rbits, pool.tbits, float(1.0 / math.sqrt(128) if sm_scale is None else sm_scale), n_splits, cus, workspace,
+                               max_q, batch.max_kv, pool.rbits, pool.tbits, float(1.0 / math.sqrt(128) if sm_scale is None else sm_scale), units, workspace,
                                need, pool.dt, pool.flags, _stream_ptr(pool.device))
     _ffi.check(rc, "pq_paged_attn")
     return (out, lse) if return_lse else out
 
 
-def paged_workspace_bytes(T: int, N: int, n_splits: int) -> int:
-    return _ffi.paged_lib().call.pq_paged_attn_workspace_bytes(T, N, n_splits)
+def paged_workspace_bytes(batch: PageBatch, N: int, n_kv_heads: int, units: int) -> int:
+    return _ffi.paged_lib().call.pq_paged_attn_workspace_bytes(batch.size, N, n_kv_heads, batch.max_q, units)
 
 
 def page_weights(q: torch.Tensor, lse: torch.Tensor, pool: PagePool, batch: PageBatch, onto: Optional[torch.Tensor] = None,

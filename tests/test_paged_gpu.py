@@ -101,13 +101,30 @@ def test_attention_of_keys_of_any_size(gpu, dtype, size):
     check_attention(c, scale=128 ** -0.5 / size / 10)
 
 
-@pytest.mark.parametrize("n_splits", [1, 2, 3, 7, 64])
-def test_attention_in_slices(gpu, n_splits):
-    """However the context is cut; slices that get no page; a workspace of the caller's."""
-    c = Cache(gpu, [900, 130, 5], [1, 1, 1], [6, 0, 0], 8, 2, torch.float16)
-    check_attention(c, n_splits=n_splits)
-    ws = torch.full((paged_workspace_bytes(c.T, c.N, n_splits) // 4,), float("nan"), device=gpu)
-    check_attention(c, n_splits=n_splits, workspace=ws)
+@pytest.mark.parametrize("new", [[1, 1, 1], [40, 3, 5]])
+@pytest.mark.parametrize("units", [0, 3, 5, 6, 7, 16, 200])
+def test_attention_in_slices(gpu, units, new):
+    """However the pages are dealt out; workgroups that get no page; a workspace of the caller's."""
+    c = Cache(gpu, [900, 130, 5], new, [6, 0, 0], 8, 2, torch.float16)
+    if units == 3 and new[0] > 1:                       # (two row tiles of the first sequence)
+        c.new[0] = 30
+        c = Cache(gpu, [900, 130, 5], c.new, [6, 0, 0], 8, 2, torch.float16)
+    check_attention(c, units=units)
+    ws = torch.full((paged_workspace_bytes(c.batch, c.N, c.Nk, units) // 4,), float("nan"), device=gpu)
+    check_attention(c, units=units, workspace=ws)
+
+
+@pytest.mark.parametrize("B", [3, 70, 130])
+def test_attention_of_many_sequences_dealt_out(gpu, B):
+    """More sequences than a wavefront has lanes, most of a page, some without new tokens, one long."""
+    r = random.Random(B)
+    kv = [r.randint(1, 200) for _ in range(B)]
+    kv[B // 2] = 3000
+    new = [r.choice([0, 1, 1, 2]) for _ in range(B)]
+    new[B // 2] = 1
+    new = [min(n, k) for n, k in zip(new, kv)]
+    for units in (2 * B, 2 * B + 17):
+        check_attention(Cache(gpu, kv, new, [(k - 1) // PAGE if k > 128 else 0 for k in kv], 4, 1, torch.bfloat16, seed=B), units=units)
 
 
 def test_attention_reads_rows_as_they_lie_and_writes_no_others(gpu):

@@ -52,12 +52,12 @@ def test_header_and_signatures_name_the_same_symbols(lib):
 
 def test_attention_arguments(lib):
     call = caller(lib.pq_validate_paged_attn, "q qr keys values codes rs rm ts tm lay qs kv ns pages vp op W Wo mask mr out lse T B N Nk mq mkv rb tb sp ws wb dt flags",
-                  dict(CACHE, q=A, qr=1024, lay=layout(), mask=None, mr=0, out=A, lse=None, sp=1, ws=None, wb=0))
+                  dict(CACHE, q=A, qr=1024, lay=layout(), mask=None, mr=0, out=A, lse=None, sp=0, ws=None, wb=0))
     assert call() == OK and call(codes=None, pages=None, rs=None) == OK and call(lse=A, mask=A, mr=1000) == OK and call(ns=None) == OK
     assert call(Wo=0, op=None) == OK and call(N=34, Nk=2, qr=34 * 128) == OK and call(dt=0) == OK
     for k in ("q", "keys", "values", "out", "qs", "kv", "vp", "op", "pages", "rs", "tm", "lay"):
         assert call(**{k: None}) == NUL, k
-    for kw in (dict(B=0), dict(N=9), dict(Nk=0), dict(mq=0), dict(mq=21), dict(mkv=0), dict(mkv=1025), dict(W=0), dict(T=0), dict(Wo=-1), dict(flags=8), dict(sp=0),
+    for kw in (dict(B=0), dict(N=9), dict(Nk=0), dict(mq=0), dict(mq=21), dict(mkv=0), dict(mkv=1025), dict(W=0), dict(T=0), dict(Wo=-1), dict(flags=8), dict(sp=-1),
                dict(sp=70000), dict(lay=layout(_8=-1)), dict(lay=layout(_10=1 << 31)), dict(T=1 << 28, N=8), dict(B=65536)):
         assert call(**kw) == SHAPE, kw
     for kw in (dict(rb=0), dict(tb=0), dict(rb=5), dict(rb=1, tb=8), dict(flags=4), dict(flags=4, rb=4, tb=3)):
@@ -69,9 +69,11 @@ def test_attention_arguments(lib):
     for k in ("q", "keys", "values", "codes", "rm", "out"):
         assert call(**{k: ODD}) == ALIGN, k
     assert call(qs=A + 2) == ALIGN and call(pages=A + 1) == ALIGN
-    need = lib.pq_paged_attn_workspace_bytes(20, 8, 3)
-    assert need == 20 * 8 * 3 * 130 * 4 and lib.pq_paged_attn_workspace_bytes(20, 8, 1) == 0
-    assert call(sp=3, ws=A, wb=need) == OK and call(sp=3, ws=A, wb=need - 1) == WS and call(sp=3) == NUL and call(sp=3, ws=ODD, wb=need) == ALIGN
+    size = lib.pq_paged_attn_workspace_bytes
+    need = size(2, 8, 2, 16, 5)
+    assert need == 5 * 2 * 128 * 130 * 4 + 16 and size(2, 8, 2, 4, 5) == 5 * 2 * 16 * 130 * 4 + 16 and size(2, 8, 2, 16, 0) == 0
+    assert call(sp=5, ws=A, wb=need) == OK and call(sp=5, ws=A, wb=need - 1) == WS and call(sp=5) == NUL and call(sp=5, ws=ODD, wb=need) == ALIGN
+    assert call(sp=1, ws=A, wb=1 << 30) == WS           # fewer than row tiles
 
 
 def test_weights_arguments(lib):
@@ -113,13 +115,13 @@ def test_seal_arguments():
     assert call(dt=2) == DTYPE and call(lay=layout(_4=8)) == STRIDE and call(keys=ODD) == ALIGN
 
 
-def test_slices(lib):
+def test_units(lib):
     plan = lib.pq_paged_attn_plan
-    assert plan(1, 32, 8, 1, 128, 256) == 1                             # a page is not cut
-    assert plan(1, 32, 8, 1, 2000, 256) == 16                           # as many slices as pages
-    assert plan(1, 32, 8, 1, 131072, 256) == 64                         # two workgroups a unit
-    assert plan(16, 32, 8, 1, 32769, 256) == 8                          # unequal sequences: room for twice the mean
-    assert plan(64, 32, 8, 1, 32769, 256) == 1 and plan(0, 1, 1, 1, 1, 256) == 1 and plan(1, 3, 2, 1, 1, 256) == 1
+    assert plan(1, 32, 8, 1, 128, 256) == 0                             # a page is not cut
+    assert plan(1, 32, 8, 1, 2000, 256) == 16                           # as many workgroups a KV head as pages
+    assert plan(1, 32, 8, 1, 131072, 256) == 64 and plan(16, 32, 8, 1, 32769, 256) == 64     # two on every unit
+    assert plan(64, 32, 8, 1, 32769, 256) == 0 and plan(1, 32, 8, 2048, 40000, 256) == 0     # the row tiles fill the device
+    assert plan(0, 1, 1, 1, 1, 256) == 0 and plan(1, 3, 2, 1, 1, 256) == 0
 
 
 def test_refusals():
@@ -149,4 +151,4 @@ def test_a_wait_state_before_every_load_to_lds(src):
             loads += 1
             assert not re.match(r"s_\S+ m0\b", previous), (previous, line)
         previous = line
-    assert loads > 0 or "rows" in src
+    assert (loads > 0) == ("chunk" in src or "weights" in src)

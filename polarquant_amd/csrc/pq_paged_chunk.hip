@@ -45,7 +45,7 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttnArgs a) {
     u32x4_a q[8];
     float row_scale = scale2;
     auto masked = [&](u32x4_a w) { return u32x4_a{(w.x ^ flip) & keep, (w.y ^ flip) & keep, (w.z ^ flip) & keep, (w.w ^ flip) & keep}; };
-    auto load_for_sealed = [&]() {          // chunk c: channels 4 c .. 4 c + 3 and 64 + 4 c .. 64 + 4 c + 3
+    auto load_for_sealed = [&]() {          // chunk c: channels 4 c, 64 + 4 c, .., 4 c + 3, 64 + 4 c + 3
         u32x4_a x[4], y[4];
         static_for<4>([&](auto I) {
             x[I] = *reinterpret_cast<const u32x4_a*>(qp + 32 * hi + 8 * I);
@@ -53,8 +53,8 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttnArgs a) {
         });
         static_for<4>([&](auto I) {
             const u32x4_a xm = masked(x[I]), ym = masked(y[I]);
-            q[2 * I] = u32x4_a{xm.x, xm.y, ym.x, ym.y};
-            q[2 * I + 1] = u32x4_a{xm.z, xm.w, ym.z, ym.w};
+            q[2 * I] = in_pairs(xm.x, xm.y, ym.x, ym.y);
+            q[2 * I + 1] = in_pairs(xm.z, xm.w, ym.z, ym.w);
         });
         if constexpr (std::is_same<T, BF16>::value) {
             float most = 0.0f;
@@ -117,7 +117,7 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttnArgs a) {
         return bits;
     };
     auto ask_codes = [&](int it, int page) {
-        const uint8_t* at = static_cast<const uint8_t*>(c.codes.at) + page * c.codes.page + h * c.codes.head;
+        const uint8_t* at = static_cast<const uint8_t*>(c.codes.at) + uniform(page) * c.codes.page + h * c.codes.head;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const int row = (it & 1) * kChunkKeys + 16 * wv + 4 * j + slot;
@@ -132,7 +132,7 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttnArgs a) {
         }
     };
     auto ask_constants = [&](int page) {
-        const int64_t at = page * c.meta.page + h * c.meta.head + 4 * i16;
+        const int64_t at = uniform(page) * c.meta.page + h * c.meta.head + 4 * i16;
         raw_rs = *reinterpret_cast<const uint2*>(c.rscale + at);
         raw_rm = *reinterpret_cast<const uint2*>(c.rmn + at);
         raw_ts = *reinterpret_cast<const uint2*>(c.tscale + at);
@@ -183,7 +183,6 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttnArgs a) {
             uint32_t w;
             if constexpr (PK6) w = unpack_codes6(static_cast<uint32_t>(((static_cast<uint64_t>(cw[2 * j + 1]) << 32) | cw[2 * j]) >> (8 * ((3 * i16) & 3))));
             else w = cw[j];
-            float rad[4];
             uint32_t cs[4];
             uint32_t r4 = (w & ~angles4) | halves4;
             if constexpr (TABLE) {
@@ -196,20 +195,27 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttnArgs a) {
 #pragma unroll
                 for (int k = 0; k < 4; k++) cs[k] = cos_sin_half(__builtin_fmaf(static_cast<float>((a4 >> (8 * k)) & 0xffu), ts[k], tm[k]));
             }
-            radii_of(r4, widths[0], widths[1], leasts[0], leasts[1], rad);
             const int row = 16 * wv + 4 * j + slot;
-            *lds_ptr<lds_u32x4>(to + row * 256 + (i16 ^ (4 * j + slot)) * 16) = quad_of_pairs(rad, cs);
+            *lds_ptr<lds_u32x4>(to + row * 256 + (i16 ^ (4 * j + slot)) * 16) = quad_of_pairs<T>(r4, widths[0], widths[1], leasts[0], leasts[1], cs);
         }
     };
     // rows to LDS; rows that are not there are copies of one that is, with weight zero
     auto ask_rows = [&](const PageStream& from, int page, int it, uint64_t bits, uint32_t to, auto KEYS) {
-        const u32x4_a at = rows_at(static_cast<const uint16_t*>(from.at) + page * from.page + h * from.head + (it & 1) * (kChunkKeys * 128));
-        const int some = bits ? __builtin_ctzll(bits) : 0;
+        constexpr bool keys = decltype(KEYS)::value;
+        const u32x4_a at = rows_at(static_cast<const uint16_t*>(from.at) + uniform(page) * from.page + h * from.head + (it & 1) * (kChunkKeys * 128));
+        to += wv * 4096;
+        if (bits == ~uint64_t{0}) {          // (without a selection a row: 40 vector instructions less)
+            const uint32_t offset = (16 * wv + slot) * 256 + (keys ? i16 ^ slot : i16 ^ (slot << 2)) * 16;
+#pragma unroll
+            for (int i = 0; i < 4; i++) rows_to_lds(at, keys ? offset ^ (64 * i) : offset, to + i * 1024, i * 1024);
+            return;
+        }
+        const int some = __builtin_ctzll(bits);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const int row = 16 * wv + 4 * i + slot, chunk = decltype(KEYS)::value ? i16 ^ (4 * i + slot) : i16 ^ (slot << 2);
+            const int row = 16 * wv + 4 * i + slot, chunk = keys ? i16 ^ (4 * i + slot) : i16 ^ (slot << 2);
             const int r = (bits >> row) & 1 ? row : some;
-            rows_to_lds(at, r * 256 + chunk * 16, to + (wv * 4 + i) * 1024);
+            rows_to_lds(at, r * 256 + chunk * 16, to + i * 1024);
         }
     };
 

@@ -146,7 +146,7 @@ __device__ __forceinline__ float both_rows_max(float v) {        // of lanes l a
 }
 
 // ---- rows to LDS ------------------------------------------------------------------------------------------------------
-// 16 bytes per lane from `offset` bytes behind a (uniform) address into 1 KiB of LDS at `lds` (uniform), lane after lane.  Not known to the
+// 16 bytes per lane from `offset` + `further` (uniform) bytes behind a (uniform) address into 1 KiB of LDS at `lds` (uniform), lane after lane.  Not known to the
 // compiler's count of loads in flight, which would make every read of LDS wait for them: rows_arrived() before the data is read, by the wavefront
 // that asked for it, and a barrier behind that before others read it.  The load reads M0 one wait state after a scalar write at the earliest; inside
 // an asm statement that is ours to see to.
@@ -156,15 +156,16 @@ __device__ __forceinline__ u32x4_a rows_at(const void* p) {
 }
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
-__device__ __forceinline__ void rows_to_lds(u32x4_a rows, uint32_t offset, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(offset), "s"(rows), "s"(uniform(static_cast<int>(lds))) : "memory", "m0");
+__device__ __forceinline__ void rows_to_lds(u32x4_a rows, uint32_t offset, uint32_t lds, uint32_t further = 0) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %3 offen lds" ::"v"(offset), "s"(rows), "s"(uniform(static_cast<int>(lds))),
+                 "s"(further) : "memory", "m0");
 }
 #pragma clang diagnostic pop
 __device__ __forceinline__ void rows_arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // ---- keys from codes --------------------------------------------------------------------------------------------------
-// A sealed key enters the score product as float16 whatever the model's type: r cos a and r sin a come out of one multiply-add each that
-// rounds to float16 (bfloat16 would take a conversion more and round eight times as coarsely).  So that nothing leaves float16's range, a
+// A sealed key enters the score product as float16 whatever the model's type: r cos a and r sin a come out of products that round to float16 (bfloat16 would take
+// conversions more and round eight times as coarsely).  So that nothing leaves float16's range, a
 // page's radii are scaled by a power of two, and so are a bfloat16 query's elements; both are taken back with the score's scale.
 constexpr int kHalfTop = 13;                  // scaled magnitudes lie below 2^13
 
@@ -178,47 +179,38 @@ __device__ __forceinline__ uint32_t cos_sin_half(float turns) {
 }
 constexpr float kTurn = 0.15915494309189535f;
 
-// r * (low half, high half of cs), rounded to float16, into the low (LO) or high half of a word
-template <bool SIN, bool LO>
-__device__ __forceinline__ void times_half(uint32_t& w, float r, uint32_t cs) {
-    if constexpr (LO && !SIN) asm("v_fma_mixlo_f16 %0, %1, %2, 0 op_sel_hi:[0,1,0]" : "=v"(w) : "v"(r), "v"(cs));
-    else if constexpr (LO) asm("v_fma_mixlo_f16 %0, %1, %2, 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]" : "=v"(w) : "v"(r), "v"(cs));
-    else if constexpr (!SIN) asm("v_fma_mixhi_f16 %0, %1, %2, 0 op_sel_hi:[0,1,0]" : "+v"(w) : "v"(r), "v"(cs));
-    else asm("v_fma_mixhi_f16 %0, %1, %2, 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]" : "+v"(w) : "v"(r), "v"(cs));
+// The word (r cos a, r sin a) of a pair in float16, from a byte that is (rho + 1/2) 2^tbits and a half of the words of widths and leasts: r = byte x width +
+// least.  For bfloat16 models r is rounded to float16 first, which is still finer than anything else there, and one packed product makes both; float16
+// models keep it in 32 bits for two more instructions.
+template <typename T, bool HIGH>
+__device__ __forceinline__ uint32_t pair_word(float byte, uint32_t width, uint32_t least, uint32_t cs) {
+    uint32_t w;
+    if constexpr (__is_same(T, BF16)) {
+        uint32_t r;
+        if constexpr (HIGH) asm("v_fma_mixlo_f16 %0, %1, %2, %3 op_sel:[0,1,1] op_sel_hi:[0,1,1]" : "=v"(r) : "v"(byte), "v"(width), "v"(least));
+        else asm("v_fma_mixlo_f16 %0, %1, %2, %3 op_sel_hi:[0,1,1]" : "=v"(r) : "v"(byte), "v"(width), "v"(least));
+        asm("v_pk_mul_f16 %0, %1, %2 op_sel_hi:[1,0]" : "=v"(w) : "v"(cs), "v"(r));
+    } else {
+        float r;
+        if constexpr (HIGH) asm("v_fma_mix_f32 %0, %1, %2, %3 op_sel:[0,1,1] op_sel_hi:[0,1,1]" : "=v"(r) : "v"(byte), "v"(width), "v"(least));
+        else asm("v_fma_mix_f32 %0, %1, %2, %3 op_sel_hi:[0,1,1]" : "=v"(r) : "v"(byte), "v"(width), "v"(least));
+        asm("v_fma_mixlo_f16 %0, %1, %2, 0 op_sel_hi:[0,1,0]" : "=v"(w) : "v"(r), "v"(cs));
+        asm("v_fma_mixhi_f16 %0, %1, %2, 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]" : "+v"(w) : "v"(r), "v"(cs));
+    }
+    return w;
 }
 
-// a * (a half of b) + (the same half of c)
-template <bool HIGH>
-__device__ __forceinline__ float times_plus_half(float a, uint32_t b, uint32_t c) {
-    float r;
-    if constexpr (HIGH) asm("v_fma_mix_f32 %0, %1, %2, %3 op_sel:[0,1,1] op_sel_hi:[0,1,1]" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-    else asm("v_fma_mix_f32 %0, %1, %2, %3 op_sel_hi:[0,1,1]" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-    return r;
+// 16 bytes of a key: pairs 4 c .. 4 c + 3 as (x y x y x y x y), from their codes without the angles' bits (halves4 in their place) and their angles'
+// cos and sin.
+template <typename T>
+__device__ __forceinline__ u32x4_a quad_of_pairs(uint32_t r4, uint32_t w0, uint32_t w1, uint32_t l0, uint32_t l1, const uint32_t (&cs)[4]) {
+    return u32x4_a{pair_word<T, false>(static_cast<float>(r4 & 0xffu), w0, l0, cs[0]), pair_word<T, true>(static_cast<float>((r4 >> 8) & 0xffu), w0, l0, cs[1]),
+                   pair_word<T, false>(static_cast<float>((r4 >> 16) & 0xffu), w1, l1, cs[2]), pair_word<T, true>(static_cast<float>(r4 >> 24), w1, l1, cs[3])};
 }
-
-// Radii of four pairs from a word of codes whose angles' bits are gone and have the lowest radius bit's half in their place: each byte is (rho + 1/2)
-// 2^tbits, exactly.  widths, leasts: float16, two words each.
-__device__ __forceinline__ void radii_of(uint32_t r4, uint32_t w0, uint32_t w1, uint32_t l0, uint32_t l1, float (&r)[4]) {
-    r[0] = times_plus_half<false>(static_cast<float>(r4 & 0xffu), w0, l0);
-    r[1] = times_plus_half<true>(static_cast<float>((r4 >> 8) & 0xffu), w0, l0);
-    r[2] = times_plus_half<false>(static_cast<float>((r4 >> 16) & 0xffu), w1, l1);
-    r[3] = times_plus_half<true>(static_cast<float>(r4 >> 24), w1, l1);
-}
-
-// 16 bytes of a key: pairs 4 c .. 4 c + 3 as (x x x x y y y y), from their radii and angles' cos and sin
-__device__ __forceinline__ u32x4_a quad_of_pairs(const float (&r)[4], const uint32_t (&cs)[4]) {
-    u32x4_a k;
-    uint32_t w[4];
-    times_half<false, true>(w[0], r[0], cs[0]);
-    times_half<false, false>(w[0], r[1], cs[1]);
-    times_half<false, true>(w[1], r[2], cs[2]);
-    times_half<false, false>(w[1], r[3], cs[3]);
-    times_half<true, true>(w[2], r[0], cs[0]);
-    times_half<true, false>(w[2], r[1], cs[1]);
-    times_half<true, true>(w[3], r[2], cs[2]);
-    times_half<true, false>(w[3], r[3], cs[3]);
-    k.x = w[0]; k.y = w[1]; k.z = w[2]; k.w = w[3];
-    return k;
+// a query's channels 4 c .. 4 c + 3 (two words) and 64 + 4 c .. (two words) in that order
+__device__ __forceinline__ u32x4_a in_pairs(uint32_t x0, uint32_t x1, uint32_t y0, uint32_t y1) {
+    return u32x4_a{__builtin_amdgcn_perm(y0, x0, 0x05040100u), __builtin_amdgcn_perm(y0, x0, 0x07060302u), __builtin_amdgcn_perm(y1, x1, 0x05040100u),
+                   __builtin_amdgcn_perm(y1, x1, 0x07060302u)};
 }
 
 // four 6-bit codes in the low 24 bits -> one a byte

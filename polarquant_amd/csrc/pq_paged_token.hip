@@ -43,7 +43,7 @@ __global__ __launch_bounds__(256, 2) void paged_token_kernel(PagedAttnArgs a) {
     const bool only = unit.slices == 1;
     const uint32_t table = uniform(lds_addr(sm) + wv * kTokenTable);
 
-    // this lane's rows, the keys they see, and their queries: 16 channels from 16 g on and 16 from 64 + 16 g on, which is the order of a key's pairs
+    // this lane's rows, the keys they see, and their queries: 16 channels from 16 g on and 16 from 64 + 16 g on
     const float scale2 = a.scale != 0.0f ? fabsf(a.scale) * kLog2e : 1.0f;
     const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u, keep = a.scale != 0.0f ? 0xffffffffu : 0u;
     int limit[NQ];
@@ -223,7 +223,6 @@ __global__ __launch_bounds__(256, 2) void paged_token_kernel(PagedAttnArgs a) {
         };
         auto key_piece = [&](uint32_t w, auto S) {
             constexpr int st = decltype(S)::value;
-            float r[4];
             uint32_t cs[4];
             uint32_t r4 = (w & ~angles4) | halves4;
             if constexpr (TABLE) {
@@ -239,8 +238,7 @@ __global__ __launch_bounds__(256, 2) void paged_token_kernel(PagedAttnArgs a) {
                     cs[k] = cos_sin_half(__builtin_fmaf(static_cast<float>((a4 >> (8 * k)) & 0xffu), t.x, t.y));
                 }
             }
-            radii_of(r4, widths[2 * st], widths[2 * st + 1], leasts[2 * st], leasts[2 * st + 1], r);
-            return quad_of_pairs(r, cs);
+            return quad_of_pairs<T>(r4, widths[2 * st], widths[2 * st + 1], leasts[2 * st], leasts[2 * st + 1], cs);
         };
         auto step = [&](auto SET, int at) {
             constexpr int set = decltype(SET)::value;
@@ -341,6 +339,10 @@ __global__ __launch_bounds__(256, 2) void paged_token_kernel(PagedAttnArgs a) {
 #pragma unroll
         for (int n = 0; n < NQ; n++) {
             sc[n] = scale2;
+            if constexpr (sealed) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) q[n][i] = in_pairs(q[n][i].x, q[n][i].y, q[n][i].z, q[n][i].w);
+            }
             if constexpr (sealed && std::is_same<T, BF16>::value) {
                 float most = 0.0f;
 #pragma unroll

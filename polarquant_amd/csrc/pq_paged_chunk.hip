@@ -13,7 +13,7 @@
 
 namespace pq {
 
-constexpr int kChunkRows = 128, kChunkKeys = 64, kChunkTile = kChunkKeys * 256, kChunkTable = 4096, kChunkAhead = 4;
+constexpr int kChunkRows = 128, kChunkKeys = 64, kChunkTile = kChunkKeys * 256, kChunkTable = 4096;
 
 template <typename T, bool PK6, bool TABLE>
 __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttnArgs a) {
@@ -175,32 +175,40 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttnArgs a) {
             }
         }
     };
-    // this wavefront's 16 keys of a sealed tile, from cw
-    auto make_keys = [&](int it, uint32_t to) {
-        const uint32_t table = lds0 + 4 * kChunkTile + ((it >> 1) & 1) * kChunkTable + i16 * 64;
+    // this wavefront's 16 keys of a sealed tile, from cw, four at a time: their lookups, then a half of a lane's four pairs at a time
+    uint32_t r4[2], cs[2][4];
+    auto look_up = [&](auto J, int it) __attribute__((always_inline)) {
+        constexpr int j = decltype(J)::value;
+        uint32_t w;
+        if constexpr (PK6) w = unpack_codes6(static_cast<uint32_t>(((static_cast<uint64_t>(cw[2 * j + 1]) << 32) | cw[2 * j]) >> (8 * ((3 * i16) & 3))));
+        else w = cw[j];
+        r4[j & 1] = (w & ~angles4) | halves4;
+        if constexpr (TABLE) {
+            const uint32_t table = lds0 + 4 * kChunkTile + ((it >> 1) & 1) * kChunkTable + i16 * 64;
+            uint32_t a4 = (w & angles4) << 2;
+            asm volatile("" : "+v"(a4), "+v"(r4[j & 1]));
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            uint32_t w;
-            if constexpr (PK6) w = unpack_codes6(static_cast<uint32_t>(((static_cast<uint64_t>(cw[2 * j + 1]) << 32) | cw[2 * j]) >> (8 * ((3 * i16) & 3))));
-            else w = cw[j];
-            uint32_t cs[4];
-            uint32_t r4 = (w & ~angles4) | halves4;
-            if constexpr (TABLE) {
-                uint32_t a4 = (w & angles4) << 2;
-                asm volatile("" : "+v"(a4), "+v"(r4));
+            for (int k = 0; k < 4; k++) cs[j & 1][k] = *lds_ptr<lds_u32>(table + ((a4 >> (8 * k)) & 0xffu) + k * 1024);
+        } else {
+            const uint32_t a4 = w & angles4;
 #pragma unroll
-                for (int k = 0; k < 4; k++) cs[k] = *lds_ptr<lds_u32>(table + ((a4 >> (8 * k)) & 0xffu) + k * 1024);
-            } else {
-                const uint32_t a4 = w & angles4;
-#pragma unroll
-                for (int k = 0; k < 4; k++) cs[k] = cos_sin_half(__builtin_fmaf(static_cast<float>((a4 >> (8 * k)) & 0xffu), ts[k], tm[k]));
-            }
-            const int row = 16 * wv + 4 * j + slot;
-            *lds_ptr<lds_u32x4>(to + row * 256 + (i16 ^ (4 * j + slot)) * 16) = quad_of_pairs<T>(r4, widths[0], widths[1], leasts[0], leasts[1], cs);
+            for (int k = 0; k < 4; k++) cs[j & 1][k] = cos_sin_half(__builtin_fmaf(static_cast<float>((a4 >> (8 * k)) & 0xffu), ts[k], tm[k]));
         }
     };
+    u32x4_a made;
+    auto make_half = [&](auto I, int it, uint32_t to) __attribute__((always_inline)) {
+        constexpr int j = decltype(I)::value >> 1, k = decltype(I)::value & 1;
+        if constexpr (k == 0 && j < 3) look_up(IC<j + 1>{}, it);
+        made[2 * k] = pair_word<T, false>(static_cast<float>((r4[j & 1] >> (16 * k)) & 0xffu), widths[k], leasts[k], cs[j & 1][2 * k]);
+        made[2 * k + 1] = pair_word<T, true>(static_cast<float>((r4[j & 1] >> (16 * k + 8)) & 0xffu), widths[k], leasts[k], cs[j & 1][2 * k + 1]);
+        if constexpr (k == 1) *lds_ptr<lds_u32x4>(to + (16 * wv + 4 * j + slot) * 256 + (i16 ^ (4 * j + slot)) * 16) = made;
+    };
+    auto make_keys = [&](int it, uint32_t to) __attribute__((always_inline)) {
+        look_up(IC<0>{}, it);
+        static_for<8>([&](auto I) { make_half(I, it, to); });
+    };
     // rows to LDS; rows that are not there are copies of one that is, with weight zero
-    auto ask_rows = [&](const PageStream& from, int page, int it, uint64_t bits, uint32_t to, auto KEYS) {
+    auto ask_rows = [&](const PageStream& from, int page, int it, uint64_t bits, uint32_t to, auto KEYS) __attribute__((always_inline)) {
         constexpr bool keys = decltype(KEYS)::value;
         const u32x4_a at = rows_at(static_cast<const uint16_t*>(from.at) + uniform(page) * from.page + h * from.head + (it & 1) * (kChunkKeys * 128));
         to += wv * 4096;
@@ -211,10 +219,13 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttnArgs a) {
             return;
         }
         const int some = __builtin_ctzll(bits);
+        const uint32_t word = static_cast<uint32_t>(bits >> (16 * wv));      // bit 4 i + slot: this lane's row of load i
+        int s4 = slot;
+        asm volatile("" : "+v"(s4));         // (nothing of this is kept in registers for its rare turn)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const int row = 16 * wv + 4 * i + slot, chunk = keys ? i16 ^ (4 * i + slot) : i16 ^ (slot << 2);
-            const int r = (bits >> row) & 1 ? row : some;
+            const int row = 16 * wv + 4 * i + s4, chunk = keys ? i16 ^ (4 * i + s4) : i16 ^ (s4 << 2);
+            const int r = (word >> (4 * i + s4)) & 1 ? row : some;
             rows_to_lds(at, r * 256 + chunk * 16, to + i * 1024);
         }
     };
@@ -225,8 +236,8 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttnArgs a) {
         for (int j = 0; j < 16; j++) o[I][j] = 0.0f;
     });
     float m = kNone, l = 0.0f;
-    uint32_t ka[8], va[4];
-    static_for<8>([&](auto I) { ka[I] = lds0 + col * 256 + ((8 * hi + I) ^ (col & 15)) * 16; });
+    const uint32_t ka = lds0 + col * 256 + ((8 * hi) ^ (col & 15)) * 16;     // chunk 8 hi; chunk 8 hi + i: i 16 exclusive-or'ed
+    uint32_t va[4];
     static_for<4>([&](auto I) {              // 16 lanes read 4 tokens x 16 channels and get them transposed
         constexpr int i = decltype(I)::value;
         const int row = 4 * hi + (i16 >> 2), chunk = 4 * i + 2 * (slot & 1) + ((lane & 3) >> 1);
@@ -234,34 +245,36 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttnArgs a) {
     });
 
     uint64_t bits = 0, bits_next = 0;
-    auto compute = [&](int it, auto BUF) {
+    // SEALED: the tile's keys are.  MAKE: the next tile's keys are made beside the score products.
+    auto compute = [&](int it, auto BUF, auto SEALED, auto MAKE) __attribute__((always_inline)) {
         constexpr int buf = decltype(BUF)::value;
+        constexpr bool make = decltype(MAKE)::value;
+        using TQ = std::conditional_t<decltype(SEALED)::value, F16, T>;
         const int key0 = it * kChunkKeys;
         floatx16_a z[2];
 #pragma unroll
         for (int u = 0; u < 2; u++)
 #pragma unroll
             for (int j = 0; j < 16; j++) z[u][j] = 0.0f;
-        auto scores = [&](auto OF) {
-            using TQ = decltype(OF);
-            u32x4_a kf[kChunkAhead][2];
-            auto k_load = [&](auto I) {
-                constexpr int i = decltype(I)::value;
-                kf[i % kChunkAhead][0] = *lds_ptr<lds_u32x4>(ka[i] + buf * kChunkTile);
-                kf[i % kChunkAhead][1] = *lds_ptr<lds_u32x4>(ka[i] + buf * kChunkTile + 32 * 256);
-            };
-            static_for<kChunkAhead>(k_load);
-            static_for<8>([&](auto I) {
-                constexpr int i = decltype(I)::value;
-                z[0] = mma32<TQ>(kf[i % kChunkAhead][0], q[i], z[0]);
-                z[1] = mma32<TQ>(kf[i % kChunkAhead][1], q[i], z[1]);
-                if constexpr (i + kChunkAhead < 8) k_load(IC<i + kChunkAhead>{});
-            });
+        constexpr int kAhead = make ? 2 : 4;                                 // steps whose keys are on their way from LDS
+        u32x4_a kf[kAhead][2];
+        auto k_load = [&](auto I) {
+            constexpr int i = decltype(I)::value;
+            kf[i % kAhead][0] = *lds_ptr<lds_u32x4>((ka ^ (16 * i)) + buf * kChunkTile);
+            kf[i % kAhead][1] = *lds_ptr<lds_u32x4>((ka ^ (16 * i)) + buf * kChunkTile + 32 * 256);
         };
-        float f = row_scale;
-        if (std::is_same<T, F16>::value || it < border) scores(F16{});
-        else scores(T{});
-        if (it < border) f *= page_scale;
+        static_for<kAhead>(k_load);
+        static_for<8>([&](auto I) {
+            constexpr int i = decltype(I)::value;
+            z[0] = mma32<TQ>(kf[i % kAhead][0], q[i], z[0]);
+            z[1] = mma32<TQ>(kf[i % kAhead][1], q[i], z[1]);
+            if constexpr (i + kAhead < 8) k_load(IC<i + kAhead>{});
+            if constexpr (make) {
+                make_half(I, it + 1, lds0 + (buf ^ 1) * kChunkTile);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        });
+        const float f = decltype(SEALED)::value ? row_scale * page_scale : row_scale;
         if (bits != ~uint64_t{0} || key0 + kChunkKeys - 1 > wave_first) {
             const int last = limit - key0 - 4 * hi;
             const uint64_t there = bits >> (4 * hi);
@@ -321,14 +334,15 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttnArgs a) {
         });
         l += sum[0] + sum[1];
     };
-    auto step = [&](int it, auto BUF) {
-        constexpr int buf = decltype(BUF)::value;
-        const bool first_half = (it & 1) == 0;
+    // One tile, and what is behind it on its way: CUR, NEXT: this tile's keys, the next one's are sealed.
+    auto step = [&](int it, auto BUF, auto CUR, auto NEXT) __attribute__((always_inline)) {
+        constexpr int buf = decltype(BUF)::value;                            // (the half of its page that a tile is)
+        constexpr bool cur = decltype(CUR)::value, sealed = decltype(NEXT)::value;
         const int p = it >> 1;
         // what is taken here was asked for a step ago, except the constants of a page's radii, two
-        if (!first_half) {
+        if constexpr (buf == 1) {
             const Ids after = taken_ids(p + 2, raw_key, raw_value);
-            if (it + 1 < it1 && it + 1 < border && next.key >= 0) take_radii();
+            if constexpr (sealed) take_radii();
             now = next;                      // (the tile that is made now is the next page's)
             next = after;
             if (it + 3 < it1 && it + 3 < border && next.key >= 0) ask_constants(next.key);
@@ -336,24 +350,23 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttnArgs a) {
             if (it + 2 < it1 && it + 2 < border && next.key >= 0) make_table(p + 1);
             asked_ids(p + 2, raw_key, raw_value);
         }
-        if (it + 1 < it1) {
-            bits_next = keys_there(it + 1, now);
-            ask_mask(it + 2);
-            const bool sealed = it + 1 < border;
-            if (bits_next) {
-                ask_rows(c.values, now.value, it + 1, bits_next, lds0 + 2 * kChunkTile + (buf ^ 1) * kChunkTile, std::false_type{});
-                if (!sealed) ask_rows(c.keys, now.key, it + 1, bits_next, lds0 + (buf ^ 1) * kChunkTile, std::true_type{});
-                else make_keys(it + 1, lds0 + (buf ^ 1) * kChunkTile);
-            }
-            const int key = first_half ? next.key : now.key;                 // of tile it + 2
+        bits_next = it + 1 < it1 ? keys_there(it + 1, now) : 0;
+        ask_mask(it + 2);
+        if (bits_next) {
+            ask_rows(c.values, now.value, it + 1, bits_next, lds0 + 2 * kChunkTile + (buf ^ 1) * kChunkTile, std::false_type{});
+            if constexpr (!sealed) ask_rows(c.keys, now.key, it + 1, bits_next, lds0 + (buf ^ 1) * kChunkTile, std::true_type{});
+        }
+        // (keys that nobody sees are made of whatever the registers hold)
+        if constexpr (sealed) make_keys(it + 1, lds0 + (buf ^ 1) * kChunkTile);
+        if (bits && it * kChunkKeys <= wave_last && row0 + wv * 32 < rows) compute(it, BUF, CUR, std::false_type{});
+        if constexpr (cur) {
+            const int key = buf ? now.key : next.key;                        // of tile it + 2
             if (it + 2 < it1 && it + 2 < border && key >= 0) ask_codes(it + 2, key);
         }
-        if (it == border && it > it0) load_for_open();
-        if (bits && it * kChunkKeys <= wave_last && row0 + wv * 32 < rows) compute(it, BUF);
         rows_arrived();
         __syncthreads();
         bits = bits_next;
-        if (!first_half) page_scale = page_scale_next;
+        if constexpr (buf == 1) page_scale = page_scale_next;
     };
 
     if (it0 < it1) {
@@ -387,9 +400,23 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttnArgs a) {
         rows_arrived();
         __syncthreads();
     }
-    for (int it = it0; it < it1; it += 2) {
-        step(it, IC<0>{});
-        if (it + 1 < it1) step(it + 1, IC<1>{});
+    using Sealed = std::true_type;
+    using Open = std::false_type;
+    int it = it0;
+    const int turn = border < it1 ? border : it1;                            // (a page's two tiles are of a kind)
+    for (; it + 2 < turn; it += 2) {
+        step(it, IC<0>{}, Sealed{}, Sealed{});
+        step(it + 1, IC<1>{}, Sealed{}, Sealed{});
+    }
+    if (it < turn) {
+        step(it, IC<0>{}, Sealed{}, Sealed{});
+        if (it + 1 < it1) step(it + 1, IC<1>{}, Sealed{}, Open{});
+        it += 2;
+        if (it < it1) load_for_open();
+    }
+    for (; it < it1; it += 2) {
+        step(it, IC<0>{}, Open{}, Open{});
+        if (it + 1 < it1) step(it + 1, IC<1>{}, Open{}, Open{});
     }
 
     l += __shfl_xor(l, 32);

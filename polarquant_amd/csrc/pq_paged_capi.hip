@@ -126,7 +126,7 @@ int pq_paged_attn_plan(int B, int N, int Nk, int max_q, int max_kv, int n_cus) {
 
 size_t pq_paged_attn_workspace_bytes(int B, int N, int Nk, int max_q, int units) {
     if (B < 1 || N < 1 || Nk < 1 || N % Nk || max_q < 1 || units < 1) return 0;
-    const size_t rows = static_cast<size_t>(units) * Nk * pq::paged_tile_rows(static_cast<int64_t>(max_q) * (N / Nk));
+    const size_t rows = static_cast<size_t>(units) * Nk * (static_cast<int64_t>(max_q) * (N / Nk) <= pq::kPagedFewRows ? 16 : pq::kPagedMostRows);
     return rows * (PQ_HEAD_DIM + 2) * sizeof(float) + static_cast<size_t>(B) * 8;
 }
 
@@ -142,7 +142,7 @@ int pq_validate_paged_attn(const void* q, int64_t q_row, const void* keys, const
     if (int rc = check_pages(codes, pages, value_pages, open_pages, Wo, rbits, tbits, flags)) return rc;
     if (int rc = check_queries(q, q_row, N, T)) return rc;
     if (int rc = check_mask(mask, mask_row, B, max_kv)) return rc;
-    const int64_t tiles = pq::paged_tiles(B, N, Nk, max_q);
+    const int64_t tiles = pq::paged_tiles(B, N, Nk, max_q, max_kv);
     if (units < 0 || units > 65535 || tiles / B > 65535 || static_cast<int64_t>(max_q) * N >= INT32_MAX) return PQ_ERR_BAD_SHAPE;
     if (!aligned(out, 16) || !aligned(lse, 4) || !aligned(workspace, 16)) return PQ_ERR_MISALIGNED;
     if (units > 0) {
@@ -175,7 +175,8 @@ int pq_paged_attn(const void* q, int64_t q_row, const void* keys, const void* va
     a.scale = scale;
     const bool packed = (flags & PQ_CODES_PACKED6) != 0;
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    return status(static_cast<int64_t>(max_q) * (N / Nk) <= pq::kPagedFewRows ? pq::launch_paged_token(a, dtype, packed, st) : pq::launch_paged_chunk(a, dtype, packed, st));
+    const int tile = pq::paged_tile_rows(static_cast<int64_t>(max_q) * (N / Nk), max_kv);
+    return status(tile == 16 ? pq::launch_paged_token(a, dtype, packed, st) : pq::launch_paged_chunk(a, dtype, packed, tile, st));
 }
 
 int pq_validate_paged_weights(const void* q, int64_t q_row, const float* lse, const void* keys, const uint8_t* codes, const void* rscale, const void* rmn,

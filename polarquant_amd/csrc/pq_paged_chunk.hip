@@ -1,6 +1,6 @@
 // Attention over the pages of a cache, for many query rows a sequence (a row: a new token and a query head).
 //
-// grid: paged_unit.  Four wavefronts with 32 rows each over 64-key tiles of K and V that
+// grid: paged_unit.  Four or eight wavefronts with 32 rows each over 64-key tiles of K and V that
 // are double-buffered in LDS; all query heads of a KV head share the tiles.  The transposed score tile S^T = K Q^T makes a row a lane, its softmax state a
 // register, and P^T the right operand of O^T = V^T P^T as it stands.
 //
@@ -13,21 +13,22 @@
 
 namespace pq {
 
-constexpr int kChunkRows = 128, kChunkKeys = 64, kChunkTile = kChunkKeys * 256, kChunkTable = 4096;
+constexpr int kChunkKeys = 64, kChunkTile = kChunkKeys * 256, kChunkTable = 4096;
 
-template <typename T, bool PK6, bool TABLE>
-__global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttnArgs a) {
+template <typename T, int WAVES, bool PK6, bool TABLE>
+__global__ __launch_bounds__(64 * WAVES, 2) void paged_chunk_kernel(PagedAttnArgs a) {
+    constexpr int kRows = 32 * WAVES, kOwn = kChunkKeys / WAVES, kLoads = kOwn / 4;        // rows; keys that a wavefront brings; loads of four rows for them
     extern __shared__ __attribute__((aligned(1024))) uint8_t sm[];           // two tiles of K, two of V, two tables
     const uint32_t lds0 = uniform(lds_addr(sm));
     const int tid = threadIdx.x, lane = tid & 63, wv = uniform(tid >> 6), col = lane & 31, hi = lane >> 5, i16 = lane & 15, slot = lane >> 4;
     const PagedCache& c = a.c;
     PagedUnit unit;
-    if (!paged_unit(c, a.units, kChunkRows, unit)) return;
+    if (!paged_unit(c, a.units, kRows, unit)) return;
     const int b = unit.b, h = blockIdx.x;
     const PagedSequence s = own_sequence(c, b);
     const int rep = c.N / c.Nk, rows = s.rows * rep, pages = ceil_div(s.kv, kPageTokens);
 
-    const int row0 = unit.tile * kChunkRows, last_row = row0 + kChunkRows - 1 < rows - 1 ? row0 + kChunkRows - 1 : rows - 1;
+    const int row0 = unit.tile * kRows, last_row = row0 + kRows - 1 < rows - 1 ? row0 + kRows - 1 : rows - 1;
     const int r = row0 + wv * 32 + col, rc = r < rows ? r : rows - 1, token = rc / rep;
     const int limit = s.past + token;                                        // last key this row sees
     const int wave_row = row0 + wv * 32 < rows - 1 ? row0 + wv * 32 : rows - 1, wave_end = wave_row + 31 < rows - 1 ? wave_row + 31 : rows - 1;
@@ -95,7 +96,7 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttnArgs a) {
     };
     Ids now, next;                          // of the page of the tile that is computed, of the one behind it
     int raw_key = -1, raw_value = -1;       // of the one behind that
-    uint32_t cw[PK6 ? 8 : 4] = {};          // codes of the tile behind the one that is made
+    uint32_t cw[PK6 ? 2 * kLoads : kLoads] = {};          // codes of the tile behind the one that is made
     uint2 raw_rs = make_uint2(0, 0), raw_rm = raw_rs, raw_ts = raw_rs, raw_tm = raw_rs;
     uint32_t widths[2] = {}, leasts[2] = {};                                 // of the radii of this lane's four pairs, float16
     float ts[4] = {}, tm[4] = {};
@@ -119,8 +120,8 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttnArgs a) {
     auto ask_codes = [&](int it, int page) {
         const uint8_t* at = static_cast<const uint8_t*>(c.codes.at) + uniform(page) * c.codes.page + h * c.codes.head;
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int row = (it & 1) * kChunkKeys + 16 * wv + 4 * j + slot;
+        for (int j = 0; j < kLoads; j++) {
+            const int row = (it & 1) * kChunkKeys + kOwn * wv + 4 * j + slot;
             if constexpr (PK6) {
                 const uint32_t* w = reinterpret_cast<const uint32_t*>(at + row * 48);
                 const int d = (3 * i16) >> 2;
@@ -166,16 +167,17 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttnArgs a) {
     };
     auto make_table = [&](int p) {
         if constexpr (TABLE) {
-            const int bin = tid >> 4;
+            const int bin = (tid >> 4) & 15;
             const uint32_t at = lds0 + 4 * kChunkTile + (p & 1) * kChunkTable + (i16 * 16 + bin) * 4;
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const float width = fourth(raw_ts, k) * kTurn;
-                *lds_ptr<lds_u32>(at + k * 1024) = cos_sin_half(__builtin_fmaf(static_cast<float>(bin) + 0.5f, width, fourth(raw_tm, k) * kTurn));
+            for (int i = 0; i < 16 / WAVES; i++) {                           // (more wavefronts than bins' sixteenths: each takes a part of the pairs)
+                const int part = uniform(tid >> 8) * (16 / WAVES);
+                const float width = (part ? fourth(raw_ts, i + 2) : fourth(raw_ts, i)) * kTurn, least = (part ? fourth(raw_tm, i + 2) : fourth(raw_tm, i)) * kTurn;
+                *lds_ptr<lds_u32>(at + (part + i) * 1024) = cos_sin_half(__builtin_fmaf(static_cast<float>(bin) + 0.5f, width, least));
             }
         }
     };
-    // this wavefront's 16 keys of a sealed tile, from cw, four at a time: their lookups, then a half of a lane's four pairs at a time
+    // this wavefront's keys of a sealed tile, from cw, four at a time: their lookups, then a half of a lane's four pairs at a time
     uint32_t r4[2], cs[2][4];
     auto look_up = [&](auto J, int it) __attribute__((always_inline)) {
         constexpr int j = decltype(J)::value;
@@ -198,33 +200,33 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttnArgs a) {
     u32x4_a made;
     auto make_half = [&](auto I, int it, uint32_t to) __attribute__((always_inline)) {
         constexpr int j = decltype(I)::value >> 1, k = decltype(I)::value & 1;
-        if constexpr (k == 0 && j < 3) look_up(IC<j + 1>{}, it);
+        if constexpr (k == 0 && j < kLoads - 1) look_up(IC<j + 1>{}, it);
         made[2 * k] = pair_word<T, false>(static_cast<float>((r4[j & 1] >> (16 * k)) & 0xffu), widths[k], leasts[k], cs[j & 1][2 * k]);
         made[2 * k + 1] = pair_word<T, true>(static_cast<float>((r4[j & 1] >> (16 * k + 8)) & 0xffu), widths[k], leasts[k], cs[j & 1][2 * k + 1]);
-        if constexpr (k == 1) *lds_ptr<lds_u32x4>(to + (16 * wv + 4 * j + slot) * 256 + (i16 ^ (4 * j + slot)) * 16) = made;
+        if constexpr (k == 1) *lds_ptr<lds_u32x4>(to + (kOwn * wv + 4 * j + slot) * 256 + (i16 ^ ((kOwn * wv + 4 * j + slot) & 15)) * 16) = made;
     };
     auto make_keys = [&](int it, uint32_t to) __attribute__((always_inline)) {
         look_up(IC<0>{}, it);
-        static_for<8>([&](auto I) { make_half(I, it, to); });
+        static_for<2 * kLoads>([&](auto I) { make_half(I, it, to); });
     };
     // rows to LDS; rows that are not there are copies of one that is, with weight zero
     auto ask_rows = [&](const PageStream& from, int page, int it, uint64_t bits, uint32_t to, auto KEYS) __attribute__((always_inline)) {
         constexpr bool keys = decltype(KEYS)::value;
         const u32x4_a at = rows_at(static_cast<const uint16_t*>(from.at) + uniform(page) * from.page + h * from.head + (it & 1) * (kChunkKeys * 128));
-        to += wv * 4096;
+        to += wv * (kOwn * 256);
         if (bits == ~uint64_t{0}) {          // (without a selection a row: 40 vector instructions less)
-            const uint32_t offset = (16 * wv + slot) * 256 + (keys ? i16 ^ slot : i16 ^ (slot << 2)) * 16;
+            const uint32_t offset = (kOwn * wv + slot) * 256 + (keys ? i16 ^ ((kOwn * wv + slot) & 15) : i16 ^ (slot << 2)) * 16;
 #pragma unroll
-            for (int i = 0; i < 4; i++) rows_to_lds(at, keys ? offset ^ (64 * i) : offset, to + i * 1024, i * 1024);
+            for (int i = 0; i < kLoads; i++) rows_to_lds(at, keys ? offset ^ (64 * i) : offset, to + i * 1024, i * 1024);
             return;
         }
         const int some = __builtin_ctzll(bits);
-        const uint32_t word = static_cast<uint32_t>(bits >> (16 * wv));      // bit 4 i + slot: this lane's row of load i
+        const uint32_t word = static_cast<uint32_t>(bits >> (kOwn * wv));    // bit 4 i + slot: this lane's row of load i
         int s4 = slot;
         asm volatile("" : "+v"(s4));         // (nothing of this is kept in registers for its rare turn)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int row = 16 * wv + 4 * i + s4, chunk = keys ? i16 ^ (4 * i + s4) : i16 ^ (s4 << 2);
+        for (int i = 0; i < kLoads; i++) {
+            const int row = kOwn * wv + 4 * i + s4, chunk = keys ? i16 ^ (row & 15) : i16 ^ (s4 << 2);
             const int r = (word >> (4 * i + s4)) & 1 ? row : some;
             rows_to_lds(at, r * 256 + chunk * 16, to + i * 1024);
         }
@@ -421,8 +423,8 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttnArgs a) {
 
     l += __shfl_xor(l, 32);
     if (unit.slices > 1) {
-        const PagedPartials part = paged_partials(a.partial, a.units, c.Nk, kChunkRows);
-        const size_t at = (static_cast<size_t>(blockIdx.y) * c.Nk + h) * kChunkRows + wv * 32 + col;
+        const PagedPartials part = paged_partials(a.partial, a.units, c.Nk, kRows);
+        const size_t at = (static_cast<size_t>(blockIdx.y) * c.Nk + h) * kRows + wv * 32 + col;
         float* out = part.state + at * 128 + 4 * hi;
         if (r < rows) {
             static_for<4>([&](auto I) {
@@ -443,27 +445,29 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedAttnArgs a) {
         if (a.lse && hi == 0) a.lse[at] = l > 0.0f ? (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f : -INFINITY;
     }
     if (a.units && h == 0 && unit.tile == 0 && unit.slice == 0 && tid == 0)
-        paged_partials(a.partial, a.units, c.Nk, kChunkRows).where[b] = make_int2(blockIdx.y, unit.slices);
+        paged_partials(a.partial, a.units, c.Nk, kRows).where[b] = make_int2(blockIdx.y, unit.slices);
 }
 
-template <typename T, bool PK6, bool TABLE>
+template <typename T, int WAVES, bool PK6, bool TABLE>
 static int launch_chunk(const PagedAttnArgs& a, hipStream_t st) {
-    constexpr int bytes = 4 * kChunkTile + (TABLE ? 2 * kChunkTable : 0);
-    const void* f = reinterpret_cast<const void*>(&paged_chunk_kernel<T, PK6, TABLE>);
+    constexpr int bytes = 4 * kChunkTile + (TABLE ? 2 * kChunkTable : 0), rows = 32 * WAVES;
+    const void* f = reinterpret_cast<const void*>(&paged_chunk_kernel<T, WAVES, PK6, TABLE>);
     if (const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, bytes); e != hipSuccess) return static_cast<int>(e);
-    const int tiles = (a.max_q * (a.c.N / a.c.Nk) + kChunkRows - 1) / kChunkRows;
-    hipLaunchKernelGGL((paged_chunk_kernel<T, PK6, TABLE>), a.units ? dim3(a.c.Nk, a.units, 1) : dim3(a.c.Nk, tiles, a.c.B), dim3(256), bytes, st, a);
+    const int tiles = (a.max_q * (a.c.N / a.c.Nk) + rows - 1) / rows;
+    hipLaunchKernelGGL((paged_chunk_kernel<T, WAVES, PK6, TABLE>), a.units ? dim3(a.c.Nk, a.units, 1) : dim3(a.c.Nk, tiles, a.c.B), dim3(64 * WAVES), bytes, st, a);
     const int err = static_cast<int>(hipGetLastError());
-    return err || a.units == 0 ? err : launch_paged_merge(a, std::is_same<T, F16>::value ? 0 : 1, kChunkRows, st);
+    return err || a.units == 0 ? err : launch_paged_merge(a, std::is_same<T, F16>::value ? 0 : 1, rows, st);
 }
 
-int launch_paged_chunk(const PagedAttnArgs& a, int dtype, bool packed, hipStream_t st) {
-    auto of = [&](auto T) {
+int launch_paged_chunk(const PagedAttnArgs& a, int dtype, bool packed, int tile_rows, hipStream_t st) {
+    auto of = [&](auto T, auto W) {
         using E = decltype(T);
-        if (packed) return launch_chunk<E, true, true>(a, st);
-        return a.c.tbits <= 4 ? launch_chunk<E, false, true>(a, st) : launch_chunk<E, false, false>(a, st);
+        constexpr int waves = decltype(W)::value;
+        if (packed) return launch_chunk<E, waves, true, true>(a, st);
+        return a.c.tbits <= 4 ? launch_chunk<E, waves, false, true>(a, st) : launch_chunk<E, waves, false, false>(a, st);
     };
-    return dtype == 0 ? of(F16{}) : of(BF16{});
+    if (tile_rows == 128) return dtype == 0 ? of(F16{}, IC<4>{}) : of(BF16{}, IC<4>{});
+    return dtype == 0 ? of(F16{}, IC<8>{}) : of(BF16{}, IC<8>{});
 }
 
 }  // namespace pq

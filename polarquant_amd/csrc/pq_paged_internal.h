@@ -33,11 +33,11 @@ struct PagedAttnArgs {
     uint16_t* out;                            // [T, N, 128]
     float* lse;                               // [T, N] or null
     float* partial;                           // the slices' states (PagedPartials)
-    int max_q, units;                         // workgroups a KV head that the pages are dealt out to; 0: a sequence is not cut
+    int max_q, units;                         // workgroups a KV head that the pages are dealt out to; 0: no row tile is cut
     float scale;
 };
 int launch_paged_token(const PagedAttnArgs& a, int dtype, bool packed, hipStream_t st);
-int launch_paged_chunk(const PagedAttnArgs& a, int dtype, bool packed, hipStream_t st);
+int launch_paged_chunk(const PagedAttnArgs& a, int dtype, bool packed, int tile_rows, hipStream_t st);
 int launch_paged_merge(const PagedAttnArgs& a, int dtype, int tile_rows, hipStream_t st);
 
 struct PagedWeightArgs {

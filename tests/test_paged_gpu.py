@@ -127,6 +127,21 @@ def test_attention_of_many_sequences_dealt_out(gpu, B):
         check_attention(Cache(gpu, kv, new, [(k - 1) // PAGE if k > 128 else 0 for k in kv], 4, 1, torch.bfloat16, seed=B), units=units)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rbits,tbits,packed,N,Nk", [(4, 4, False, 8, 2), (3, 3, True, 14, 2), (3, 5, False, 8, 8)])
+@pytest.mark.parametrize("units,masked", [(None, False), (0, True), (80, True), (200, False)])
+def test_attention_of_batches_that_may_be_long(gpu, dtype, rbits, tbits, packed, N, Nk, units, masked):
+    """Of many new tokens and up to 4200 in all: rows in the largest tiles, also for the short sequences of the batch."""
+    kv, new = [1, 128, 640, 515, 0, 900, 77, 300], [1, 1, 33, 130, 0, 300, 77, 0]
+    c = Cache(gpu, kv, new, [0, 0, 4, 3, 0, 4, 0, 2], N, Nk, dtype, rbits, tbits, packed, seed=N, wide=25)
+    b = c.batch
+    c.batch = PageBatch(b.q_start, b.kv_len, b.n_sealed, b.pages, b.open_pages, b.max_q, 4200)
+    if masked:
+        c.mask = (torch.rand(8, 4200, generator=torch.Generator(device=gpu).manual_seed(2), device=gpu) < 0.6).to(torch.uint8)
+        c.mask[5, :300] = 0
+    check_attention(c, batch=c.batch, units=units)
+
+
 def test_attention_reads_rows_as_they_lie_and_writes_no_others(gpu):
     """Queries that are a slice of a projection's output; rows of no sequence; tables wider than what is held."""
     c = Cache(gpu, [300, 200], [3, 2], [1, 0], 4, 2, torch.bfloat16, extra_rows=4, wide=3)

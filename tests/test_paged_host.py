@@ -71,7 +71,7 @@ def test_attention_arguments(lib):
     assert call(qs=A + 2) == ALIGN and call(pages=A + 1) == ALIGN
     size = lib.pq_paged_attn_workspace_bytes
     need = size(2, 8, 2, 16, 5)
-    assert need == 5 * 2 * 128 * 130 * 4 + 16 and size(2, 8, 2, 4, 5) == 5 * 2 * 16 * 130 * 4 + 16 and size(2, 8, 2, 16, 0) == 0
+    assert need == 5 * 2 * 256 * 130 * 4 + 16 and size(2, 8, 2, 4, 5) == 5 * 2 * 16 * 130 * 4 + 16 and size(2, 8, 2, 16, 0) == 0
     assert call(sp=5, ws=A, wb=need) == OK and call(sp=5, ws=A, wb=need - 1) == WS and call(sp=5) == NUL and call(sp=5, ws=ODD, wb=need) == ALIGN
     assert call(sp=1, ws=A, wb=1 << 30) == WS           # fewer than row tiles
 

@@ -34,15 +34,46 @@ __global__ __launch_bounds__(256, 2) void paged_weights_kernel(PagedWeightArgs a
         return;
     }
     const uint32_t lds0 = lds_addr(sm);
-    auto fetch = [&](int tile, int buf) {
-        const int t0 = tile * kWeightRows / rep;
-        const u32x4_a qb = rows_at(a.q + (s.first + t0) * a.q_row + h * rep * 128);
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int row = (wv * 4 + i) * 4 + (lane >> 4), chunk = (lane & 15) ^ (row & 15);
-            int r = tile * kWeightRows + row;
-            r = r < rows ? r : rows - 1;
-            rows_to_lds(qb, static_cast<uint32_t>(r / rep - t0) * static_cast<uint32_t>(2 * a.q_row) + (r % rep) * 256 + chunk * 16, lds0 + buf * kWeightTile + (wv * 4 + i) * 1024);
+    // A row is a token and a query head, r / rep and r % rep.  From one tile to the next a lane's token goes on by 64 / rep, with its base, and its head by 64 % rep:
+    // nothing of it is left to the lanes where rep divides 64.
+    const int step_t = kWeightRows / rep, step_head = kWeightRows % rep, t0 = tile0 * kWeightRows / rep;
+    const uint32_t token_bytes = 2 * static_cast<uint32_t>(a.q_row);
+    const uint16_t* base = a.q + (s.first + t0) * a.q_row + h * rep * 128;
+    const float* lse_base = a.lse + (s.first + t0) * static_cast<int64_t>(c.N) + h * rep;
+    int head[6];                              // of this lane's four rows that it brings, and two whose scores it has
+    uint32_t offset[6];                       // of their queries and log sums from the bases
+    auto row_of = [&](int i) { return i < 4 ? (wv * 4 + i) * 4 + (lane >> 4) : 32 * (i - 4) + col; };
+    auto offset_of = [&](int i, int t, int hd) { return i < 4 ? t * token_bytes + hd * 256 : static_cast<uint32_t>(4 * (t * c.N + hd)); };
+    static_for<6>([&](auto I) {
+        const int r = tile0 * kWeightRows + row_of(I);
+        head[I] = r % rep;
+        offset[I] = offset_of(I, r / rep - t0, head[I]);
+    });
+    float raw[2];                             // log sums of the rows of the tile that is on its way
+    auto fetch = [&](int tile, int buf) __attribute__((always_inline)) {
+        if ((tile + 1) * kWeightRows > rows) {                               // (the last row in place of those behind it)
+            const int t = s.rows - 1 - t0 - (tile - tile0) * step_t;
+            static_for<6>([&](auto I) {
+                if (tile * kWeightRows + row_of(I) >= rows) offset[I] = offset_of(I, t, rep - 1);
+            });
+        }
+        const u32x4_a qb = rows_at(base);
+        static_for<4>([&](auto I) {
+            constexpr int i = decltype(I)::value;
+            const int row = (wv * 4 + i) * 4 + (lane >> 4);
+            rows_to_lds(qb, offset[i] + ((lane & 15) ^ (row & 15)) * 16, lds0 + buf * kWeightTile + (wv * 4 + i) * 1024);
+        });
+        raw[0] = *reinterpret_cast<const float*>(reinterpret_cast<const char*>(lse_base) + offset[4]);
+        raw[1] = *reinterpret_cast<const float*>(reinterpret_cast<const char*>(lse_base) + offset[5]);
+        base += step_t * a.q_row;
+        lse_base += step_t * static_cast<int64_t>(c.N);
+        if (step_head) {
+            static_for<6>([&](auto I) {
+                head[I] += step_head;
+                const bool over = head[I] >= rep;
+                head[I] -= over ? rep : 0;
+                offset[I] += offset_of(I, 0, step_head) + (over ? offset_of(I, 1, 0) - offset_of(I, 0, rep) : 0u);
+            });
         }
     };
     fetch(tile0, 0);
@@ -114,50 +145,58 @@ __global__ __launch_bounds__(256, 2) void paged_weights_kernel(PagedWeightArgs a
 #pragma unroll
         for (int i = 0; i < 8; i++) kl[i] = u32x4_a{0u, 0u, 0u, 0u};
     }
-    const float scale2 = a.scale * kLog2e;
-    float total = 0.0f;
+    if (a.scale == 0.0f) {                    // (every score is zero)
+        static_for<8>([&](auto I) { kf[I] = kl[I] = u32x4_a{0u, 0u, 0u, 0u}; });
+    }
+    const float scale2 = a.scale != 0.0f ? a.scale * kLog2e : 1.0f, least = scale2 > 0.0f ? -INFINITY : INFINITY;       // a score whose weight is zero
+    float total[2] = {0.0f, 0.0f};
     rows_arrived();
     __syncthreads();
-    for (int tile = tile0; tile < tiles; tile++) {
-        const int buf = (tile - tile0) & 1;
-        if (tile + 1 < tiles) fetch(tile + 1, buf ^ 1);
+    const int whole = ((max(key0 + 31 - s.past, 0) * rep) + kWeightRows - 1) / kWeightRows;      // the first tile whose rows see all of this wavefront's keys
+    auto walk = [&](auto SEALED) __attribute__((always_inline)) {
+        constexpr int products = decltype(SEALED)::value ? 16 : 8;
+        for (int tile = tile0; tile < tiles; tile++) {
+            const int buf = (tile - tile0) & 1;
+            const float log_sum[2] = {raw[0] * kLog2e, raw[1] * kLog2e};
+            if (tile + 1 < tiles) fetch(tile + 1, buf ^ 1);
+            floatx16_a z[2];
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const int r = tile * kWeightRows + 32 * u + col, rc = r < rows ? r : rows - 1, t = rc / rep;
-            float sum2 = a.lse[static_cast<int64_t>(s.first + t) * c.N + h * rep + rc % rep] * kLog2e;
-            sum2 = r < rows && sum2 != -INFINITY ? sum2 : INFINITY;          // (no row there, or one that saw nothing: no weight)
-            floatx16_a z;
+            for (int u = 0; u < 2; u++)
 #pragma unroll
-            for (int j = 0; j < 16; j++) z[j] = 0.0f;
-            u32x4_a q[8];
+                for (int j = 0; j < 16; j++) z[u][j] = 0.0f;
+            static_for<8>([&](auto I) {
+                constexpr int i = decltype(I)::value;
 #pragma unroll
-            for (int i = 0; i < 8; i++) q[i] = *lds_ptr<lds_u32x4>(lds0 + buf * kWeightTile + (32 * u + col) * 256 + ((8 * hi + i) ^ (col & 15)) * 16);
-#pragma unroll
-            for (int i = 0; i < 8; i++) z = mma32<T>(kf[i], q[i], z);
-            if (sealed) {
-#pragma unroll
-                for (int i = 0; i < 8; i++) z = mma32<T>(kl[i], q[i], z);
-            }
-            const int first_limit = s.past + (tile * kWeightRows + 32 * u) / rep;
-            if (bits != 0xffffffffu || key0 + 31 > first_limit) {
-                const int last = s.past + t - key0 - 4 * hi;
-                const uint32_t there = bits >> (4 * hi);
-#pragma unroll
-                for (int j = 0; j < 16; j++) {
-                    const int e = 8 * (j >> 2) + (j & 3);
-                    const float w = exp2_hw(__builtin_fmaf(z[j], scale2, -sum2));
-                    total += e <= last && (there >> e & 1) ? w : 0.0f;
+                for (int u = 0; u < 2; u++) {
+                    const u32x4_a q = *lds_ptr<lds_u32x4>(lds0 + buf * kWeightTile + (32 * u + col) * 256 + ((8 * hi + i) ^ (col & 15)) * 16);
+                    z[u] = mma32<T>(kf[i], q, z[u]);
+                    if constexpr (products == 16) z[u] = mma32<T>(kl[i], q, z[u]);
                 }
-            } else {
+            });
 #pragma unroll
-                for (int j = 0; j < 16; j++) total += exp2_hw(__builtin_fmaf(z[j], scale2, -sum2));
+            for (int u = 0; u < 2; u++) {
+                const int r = tile * kWeightRows + 32 * u + col;
+                if (bits != 0xffffffffu || tile < whole) {
+                    const int last = s.past + (r < rows ? r : rows - 1) / rep - key0 - 4 * hi;
+                    const uint32_t there = bits >> (4 * hi);
+#pragma unroll
+                    for (int j = 0; j < 16; j++) {
+                        const int e = 8 * (j >> 2) + (j & 3);
+                        z[u][j] = e <= last && (there >> e & 1) ? z[u][j] : least;
+                    }
+                }
+                const float sum2 = r < rows && log_sum[u] != -INFINITY ? log_sum[u] : INFINITY;
+#pragma unroll
+                for (int j = 0; j < 16; j++) total[j & 1] += exp2_hw(__builtin_fmaf(z[u][j], scale2, -sum2));
             }
+            rows_arrived();
+            __syncthreads();
         }
-        rows_arrived();
-        __syncthreads();
-    }
-    total = wave_sum(total);
-    if (lane == 0) sums[wv] = total;
+    };
+    if (sealed) walk(IC<1>{});
+    else walk(IC<0>{});
+    const float own = wave_sum(total[0] + total[1]);
+    if (lane == 0) sums[wv] = own;
     __syncthreads();
     if (tid == 0) a.weights[entry] = had + ((sums[0] + sums[1]) + (sums[2] + sums[3]));
 }

@@ -374,6 +374,58 @@ PyObject* plain_rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
                          (long long)t.stride(1), (long long)t.stride(2), (long long)t.stride(3), dt);
 }
 
+// Packed rows [T, heads * 128] or [T, heads, 128] as the paged cache's kernels read them: of the pool's type, on its GPU.
+struct Packed {
+    int64_t row = 0, rows = 0, heads = 0;
+    bool take(PyObject* o, const at::Tensor& keys) {
+        if (!plain_tensor(o)) return false;
+        const at::Tensor& t = THPVariable_Unpack(o);
+        if (t.layout() != at::kStrided || !t.has_storage() || !t.is_cuda() || t.device() != keys.device() || t.scalar_type() != keys.scalar_type()) return false;
+        const int64_t dim = t.dim();
+        if ((dim != 2 && dim != 3) || t.numel() == 0 || t.stride(dim - 1) != 1) return false;
+        if (dim == 3 && (t.size(2) != 128 || (t.size(1) > 1 && t.stride(1) != 128))) return false;
+        const int64_t width = dim == 2 ? t.size(1) : t.size(1) * 128;
+        rows = t.size(0);
+        row = rows > 1 ? t.stride(0) : width;
+        heads = width / 128;
+        return width % 128 == 0 && row % 8 == 0 && row >= width && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
+    }
+};
+
+// plain_packed(a pool's keys, q) -> (row stride, T, heads) of queries with whole groups of heads that nothing has to be asked or copied of, or None
+PyObject* plain_packed(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    Packed q;
+    if (n != 2 || !plain_tensor(args[0])) Py_RETURN_NONE;
+    const at::Tensor& keys = THPVariable_Unpack(args[0]);
+    if (!q.take(args[1], keys) || q.heads % keys.size(1)) Py_RETURN_NONE;
+    return Py_BuildValue("(LLL)", (long long)q.row, (long long)q.rows, (long long)q.heads);
+}
+
+// plain_append(a pool's keys, q, k, v, cos, sin, norm of queries, norm of keys) -> (row strides of q, k and v, T, heads, rows of the table), or None; norms
+// may be None
+PyObject* plain_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    Packed q, k, v;
+    if (n != 8 || !plain_tensor(args[0])) Py_RETURN_NONE;
+    const at::Tensor& keys = THPVariable_Unpack(args[0]);
+    if (!q.take(args[1], keys) || !k.take(args[2], keys) || !v.take(args[3], keys)) Py_RETURN_NONE;
+    if (q.heads % keys.size(1) || k.heads != keys.size(1) || v.heads != k.heads || k.rows != q.rows || v.rows != q.rows) Py_RETURN_NONE;
+    Plain p;
+    p.device = keys.device();
+    const at::Tensor *cos = p.take(args[4], 2), *sin = p.take(args[5], 2);
+    if (!p.ok || cos->size(1) != 128 || cos->sizes() != sin->sizes()) Py_RETURN_NONE;
+    p.type(cos, keys.scalar_type());
+    p.type(sin, keys.scalar_type());
+    for (int i = 6; i < 8 && p.ok; i++) {
+        if (args[i] == Py_None) continue;
+        if (const at::Tensor* m = p.take(args[i], 1)) {
+            p.type(m, keys.scalar_type());
+            p.ok = p.ok && m->size(0) == 128;
+        }
+    }
+    if (!p.ok) Py_RETURN_NONE;
+    return Py_BuildValue("(LLLLLL)", (long long)q.row, (long long)k.row, (long long)v.row, (long long)q.rows, (long long)q.heads, (long long)cos->size(0));
+}
+
 // empty(like, type, *sizes): torch.empty on like's device, of its type (0), uint8 (1), int32 (2) or float32 (3), in half the time
 PyObject* empty(PyObject*, PyObject* const* args, Py_ssize_t n) {
     static constexpr at::ScalarType kTypes[] = {at::kHalf, at::kByte, at::kInt, at::kFloat};
@@ -420,6 +472,8 @@ PyMethodDef methods[] = {
     {"plain_scores", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&asked<plain_scores>)), METH_FASTCALL, nullptr},
     {"plain_cache", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&asked<plain_cache>)), METH_FASTCALL, nullptr},
     {"plain_rows", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&asked<plain_rows>)), METH_FASTCALL, nullptr},
+    {"plain_packed", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&asked<plain_packed>)), METH_FASTCALL, nullptr},
+    {"plain_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&asked<plain_append>)), METH_FASTCALL, nullptr},
     {"empty", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&empty)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 

@@ -92,6 +92,13 @@ class PageBatch:
                     "counts and pages of a batch of %d must be contiguous int32 tensors on %s, %d pages wide", B, self.device, self.width)
         _refuse(not 0 < self.max_kv <= PAGE * self.width, "max_kv must be within the %d pages of the table", self.width)
 
+    def _with(self, kv_len: torch.Tensor, n_sealed: torch.Tensor, pages: torch.Tensor) -> "PageBatch":
+        """This batch with tensors that lie as its own do."""
+        other = object.__new__(PageBatch)
+        other.__dict__.update(self.__dict__)
+        other.kv_len, other.n_sealed, other.pages, other.value_pages = kv_len, n_sealed, pages, pages
+        return other
+
 
 def _heads(t: torch.Tensor, name: str, n: Optional[int] = None) -> Tuple[torch.Tensor, int, int, int]:
     """Rows [T, n * 128] or [T, n, 128] as they lie -> (tensor, row stride, T, n); copied where the kernels could not read them."""
@@ -107,6 +114,27 @@ def _heads(t: torch.Tensor, name: str, n: Optional[int] = None) -> Tuple[torch.T
 def _same(pool: PagePool, batch: PageBatch, *ts):
     _refuse(batch.device != pool.device or any(t is not None and t.device != pool.device for t in ts), "tensors must be on the pool's device, %s", pool.device)
     _refuse(batch.q_start is None, "the batch does not say which rows are whose (q_start)")
+
+
+def _queries(q: torch.Tensor, pool: PagePool, batch: PageBatch, *ts) -> Tuple[torch.Tensor, int, int, int]:
+    """(q, its row stride, T, N), of the pool's type and on its device with the others; the common call's host side is one question."""
+    _gpu(q)
+    plain = _calls.plain_packed(pool.keys, q)
+    if any(t is not None for t in ts):
+        _same(pool, batch, *ts)
+    if plain is not None and batch.q_start is not None and batch.device == pool.device:
+        return q, *plain
+    _same(pool, batch, q)
+    q, q_row, T, N = _heads(q, "q")
+    _refuse(q.dtype != pool.dtype or N % pool.n_kv_heads != 0, "q must be %s, with a multiple of %d heads", pool.dtype, pool.n_kv_heads)
+    return q, q_row, T, N
+
+
+def _output(out: Optional[torch.Tensor], like: torch.Tensor, T: int, N: int) -> torch.Tensor:
+    if out is None:
+        return _calls.empty(like, 0, T, N, 128)
+    _refuse(out.dtype != like.dtype or tuple(out.shape) != (T, N, 128) or not out.is_contiguous(), "out must be a contiguous [%d, %d, 128]", T, N)
+    return out
 
 
 def _mask(mask: Optional[torch.Tensor], batch: PageBatch):
@@ -126,25 +154,28 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: 
     table; a token's row is its place in its sequence, or positions[t] (int32 [T]: a sequence from which pages were evicted has its own); beyond
     the table the nearest.  All in float32, rounded once.  Rows from q_start[-1] on are left as `out` has them."""
     _gpu(q)
-    _same(pool, batch, q, k, v, cos, sin, q_norm, k_norm, positions, out)
     Nk = pool.n_kv_heads
-    q, q_row, T, N = _heads(q, "q")
-    k, k_row, Tk, _ = _heads(k, "k", Nk)
-    v, v_row, Tv, _ = _heads(v, "v", Nk)
-    _refuse(Tk != T or Tv != T or N % Nk != 0, "q, k and v must have as many rows, and whole groups of heads")
-    for t in (k, v, cos, sin, q_norm, k_norm):
-        _refuse(t is not None and t.dtype != pool.dtype, "q, k, v, angles and norms must be %s", pool.dtype)
-    _refuse(q.dtype != pool.dtype, "q must be %s", pool.dtype)
-    _refuse(cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] != 128, "cos and sin must be [rows, 128]")
-    cos, sin = cos.contiguous(), sin.contiguous()
-    for t in (q_norm, k_norm):
-        _refuse(t is not None and (t.numel() != 128 or not t.is_contiguous()), "norms must be [128]")
+    plain = _calls.plain_append(pool.keys, q, k, v, cos, sin, q_norm, k_norm)
+    if plain is not None and batch.q_start is not None and batch.device == pool.device:      # nothing to ask or to copy
+        q_row, k_row, v_row, T, N, table = plain
+    else:
+        _same(pool, batch, q, k, v, cos, sin, q_norm, k_norm)
+        q, q_row, T, N = _heads(q, "q")
+        k, k_row, Tk, _ = _heads(k, "k", Nk)
+        v, v_row, Tv, _ = _heads(v, "v", Nk)
+        _refuse(Tk != T or Tv != T or N % Nk != 0, "q, k and v must have as many rows, and whole groups of heads")
+        for t in (q, k, v, cos, sin, q_norm, k_norm):
+            _refuse(t is not None and t.dtype != pool.dtype, "q, k, v, angles and norms must be %s", pool.dtype)
+        _refuse(cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] != 128, "cos and sin must be [rows, 128]")
+        cos, sin, table = cos.contiguous(), sin.contiguous(), cos.shape[0]
+        for t in (q_norm, k_norm):
+            _refuse(t is not None and (t.numel() != 128 or not t.is_contiguous()), "norms must be [128]")
+    if positions is not None or out is not None:
+        _same(pool, batch, positions, out)
     _refuse(positions is not None and (positions.dtype != torch.int32 or positions.numel() != T or not positions.is_contiguous()), "positions must be int32 [T]")
-    if out is None:
-        out = _calls.empty(q, 0, T, N, 128)
-    _refuse(out.dtype != pool.dtype or tuple(out.shape) != (T, N, 128) or not out.is_contiguous(), "out must be a contiguous [%d, %d, 128]", T, N)
+    out = _output(out, q, T, N)
     with _on_device(pool.device):
-        rc = _ffi.paged_lib().call.pq_paged_append(q, q_row, k, k_row, v, v_row, cos, sin, cos.shape[0], positions, q_norm, k_norm, float(eps), out, pool.keys,
+        rc = _ffi.paged_lib().call.pq_paged_append(q, q_row, k, k_row, v, v_row, cos, sin, table, positions, q_norm, k_norm, float(eps), out, pool.keys,
                                                    pool.values, pool.layout, batch.q_start, batch.kv_len, batch.n_sealed, batch.value_pages, batch.open_pages,
                                                    batch.width, batch.open_width, T, batch.size, N, Nk, min(batch.max_q, T), batch.max_kv, pool.dt,
                                                    _stream_ptr(pool.device))
@@ -171,10 +202,7 @@ def paged_attention(q: torch.Tensor, pool: PagePool, batch: PageBatch, attention
     exponentials (for `page_weights`).  The pages are dealt out to `units` workgroups a KV head (0: no
     sequence is cut) through `workspace` (float32, of paged_workspace_bytes(batch, N, Nk, units); by default memory of this call alone, so calls of several streams and
     graphs do not meet)."""
-    _gpu(q)
-    _same(pool, batch, q, attention_mask, workspace, out)
-    q, q_row, T, N = _heads(q, "q")
-    _refuse(q.dtype != pool.dtype or N % pool.n_kv_heads != 0, "q must be %s, with a multiple of %d heads", pool.dtype, pool.n_kv_heads)
+    q, q_row, T, N = _queries(q, pool, batch, attention_mask, workspace, out)
     mask, mask_row = _mask(attention_mask, batch)
     lib, max_q, cus = _ffi.paged_lib().call, min(batch.max_q, T), _num_cus(pool.device)
     if units is None:
@@ -184,9 +212,7 @@ def paged_attention(q: torch.Tensor, pool: PagePool, batch: PageBatch, attention
         workspace = _calls.empty(q, 3, need // 4) if need else None
     else:
         _refuse(workspace.dtype != torch.float32 or not workspace.is_contiguous() or workspace.numel() * 4 < need, "workspace must be float32 with %d bytes", need)
-    if out is None:
-        out = _calls.empty(q, 0, T, N, 128)
-    _refuse(out.dtype != pool.dtype or tuple(out.shape) != (T, N, 128) or not out.is_contiguous(), "out must be a contiguous [%d, %d, 128]", T, N)
+    out = _output(out, q, T, N)
     lse = _calls.empty(q, 3, T, N) if return_lse else None
     with _on_device(pool.device):
         rc = lib.pq_paged_attn(q, q_row, pool.keys, pool.values, pool.codes, *pool.meta, pool.layout, batch.q_start, batch.kv_len, batch.n_sealed, batch.pages,
@@ -205,10 +231,7 @@ def page_weights(q: torch.Tensor, lse: torch.Tensor, pool: PagePool, batch: Page
                  attention_mask: Optional[torch.Tensor] = None, sm_scale: Optional[float] = None) -> torch.Tensor:
     """The attention weight that the rows of q [T, N, 128] give to each page, summed over rows, tokens and a KV head's query heads: float32 [B, Nk, W], plus
     `onto`.  lse [T, N] as `paged_attention` returns it for the same q, mask and scale; a row of -inf gives none."""
-    _gpu(q)
-    _same(pool, batch, q, lse, onto, attention_mask)
-    q, q_row, T, N = _heads(q, "q")
-    _refuse(q.dtype != pool.dtype or N % pool.n_kv_heads != 0, "q must be %s, with a multiple of %d heads", pool.dtype, pool.n_kv_heads)
+    q, q_row, T, N = _queries(q, pool, batch, lse, onto, attention_mask)
     _refuse(lse.dtype != torch.float32 or tuple(lse.shape) != (T, N) or not lse.is_contiguous(), "lse must be a contiguous float32 [%d, %d]", T, N)
     shape = (batch.size, pool.n_kv_heads, batch.width)
     _refuse(onto is not None and (onto.dtype != torch.float32 or tuple(onto.shape) != shape or not onto.is_contiguous()), "onto must be float32 %s", shape)
@@ -242,4 +265,4 @@ def evict_pages(weights: torch.Tensor, batch: PageBatch, keep: int, sinks: int =
         rc = _ffi.paged_lib().call.pq_evict_pages(weights, batch.pages, batch.n_sealed, batch.kv_len, B, weights.shape[1], W, keep, sinks, pages, n_sealed, kv_len,
                                                   left, freed, _stream_ptr(batch.device))
     _ffi.check(rc, "pq_evict_pages")
-    return PageBatch(batch.q_start, kv_len, n_sealed, pages, batch.open_pages, batch.max_q, batch.max_kv), left, freed
+    return batch._with(kv_len, n_sealed, pages), left, freed

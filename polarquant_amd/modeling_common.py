@@ -14,7 +14,9 @@ kernels, and the cache tensors handed back in the tuple are views into a
 pre-allocated per-layer arena, so appending a token or a quantized group is O(1)
 instead of a torch.cat of the whole cache (reference :86-90,98).  The tuple is a
 `PolarCache` (a tuple subclass) that remembers its arena; a plain tuple in the
-reference's format is accepted too and is copied into a fresh arena.
+reference's format is accepted too and is copied into a fresh arena.  Several new
+tokens behind a cache (a prompt in portions, a conversation's next turn) are taken
+by the polar variant with half-precision values; the reference refuses them.
 
 The modules are self-contained torch.nn modules whose parameter names match the
 HF Llama / Qwen2 checkpoints (model.layers.N.self_attn.q_proj.weight, ...), so a
@@ -33,6 +35,7 @@ from torch.utils._device import DeviceContext
 
 from ._ffi import calls as _calls
 from .attention import polar_decode_attention, polar_decode_attention_v4, prompt_attention, prompt_attention_takes
+from .paged import PageBatch, PagePool, paged_attention
 from .quantize import quantize_and_pack_nbit
 from .values import quantize_values
 
@@ -342,6 +345,39 @@ class _Arena:
                                group_offset=self.n_groups, eager_gpu=self.eager_gpu)
         self.n_groups += n
 
+    def attend(self, q, k, v, mask, scale):
+        """Rotated queries, keys and values [B, heads, L, 128] of a portion of new tokens -> [B, L, N, 128]: each token's attention over everything that is cached and
+        over the portion up to itself; the cache then holds the portion.  The arena is read as pages of 128 tokens where it lies: a sequence's are as far from
+        the next one's as its heads' are together.  Its open pages are the residual window with the portion behind it."""
+        B, Nk, L, dev, held = self.B, self.Nk, q.shape[2], self.device, self.n_resid + q.shape[2]
+        self.reserve(self.kv_len + L)
+        n_open = (held + GROUP - 1) // GROUP
+        fresh = torch.empty(B, Nk, n_open * GROUP, 128, dtype=self.dtype, device=dev)
+        fresh[:, :, :self.n_resid] = self.kres[:, :, :self.n_resid]
+        fresh[:, :, self.n_resid:held] = k
+        self.v[:, :, self.kv_len:self.kv_len + L] = v
+        self.kv_len += L
+
+        def pages_of(t, cap, width):
+            rows = t.numel() // (B * Nk * cap * width)
+            return t.as_strided(((B - 1) * Nk * cap + cap, Nk, rows, width), (rows * width, cap * rows * width, width, 1))
+
+        def table(cap, n):
+            return torch.arange(0, B * Nk * cap, Nk * cap, dtype=torch.int32, device=dev)[:, None] + torch.arange(n, dtype=torch.int32, device=dev)
+        vcap, n = self.vcap // GROUP, (self.kv_len + GROUP - 1) // GROUP
+        pool = PagePool(pages_of(fresh, n_open, 128), pages_of(self.v, vcap, 128), pages_of(self.codes, self.gcap, self.row), *(pages_of(m, self.gcap, 64) for m in self.meta),
+                        rbits=self.rbits, tbits=self.tbits)
+        batch = PageBatch(torch.arange(0, B * L + 1, L, dtype=torch.int32, device=dev), torch.full((B,), self.kv_len, dtype=torch.int32, device=dev),
+                          torch.full((B,), self.n_groups, dtype=torch.int32, device=dev), table(self.gcap, n), table(n_open, n_open), L, self.kv_len,
+                          value_pages=table(vcap, n))
+        out = paged_attention(q.transpose(1, 2).reshape(B * L, -1, 128), pool, batch, attention_mask=mask, sm_scale=scale)
+        full = held - held % GROUP
+        if full:
+            self.quantize_into(fresh[:, :, :full])
+        self.n_resid = held - full
+        self.kres[:, :, :self.n_resid] = fresh[:, :, full:held]
+        return out.view(B, L, -1, 128)
+
     def as_tuple(self) -> "PolarCache":
         kf = self.kres[:, :, :self.n_resid] if self.n_resid else None
         if self.n_groups:
@@ -468,8 +504,12 @@ class PolarGroupAttention(nn.Module):
                 arena.quantize_into(arena.kres)
                 arena.n_resid = 0
             past_key_value = arena.as_tuple()                              # :101
+        # a further portion of a prompt, or a conversation's next turn, behind a cache (the reference takes a prompt in one call only)
+        elif past_key_value is not None:
+            arena = self._arena_of(past_key_value, query_states.dtype, query_states.device)
+            attn_output = arena.attend(query_states, key_states, value_states, _mask_u8(attention_mask), 1.0 / math.sqrt(self.head_dim))
+            past_key_value = arena.as_tuple()
         else:            # pre-filling (:102-128)
-            assert past_key_value is None
             kv_seq_len = key_states.shape[2]
             attn_output = _prefill_attention(query_states, key_states, value_states, attention_mask,
                                              self.num_key_value_groups, self.is_causal)

@@ -16,6 +16,7 @@ constexpr int kWeightRows = 64, kWeightTile = kWeightRows * 256;
 template <typename T, bool PK6>
 __global__ __launch_bounds__(256, 2) void paged_weights_kernel(PagedWeightArgs a) {
     __shared__ __attribute__((aligned(1024))) uint8_t sm[2 * kWeightTile];
+    __shared__ __attribute__((aligned(16))) float constants[4 * 2 * 64 * 4];
     __shared__ float sums[4];
     const PagedCache& c = a.c;
     const int tid = threadIdx.x, lane = tid & 63, wv = uniform(tid >> 6), col = lane & 31, hi = lane >> 5;
@@ -91,7 +92,15 @@ __global__ __launch_bounds__(256, 2) void paged_weights_kernel(PagedWeightArgs a
     if (sealed) {
         const uint8_t* row = static_cast<const uint8_t*>(c.codes.at) + kp * c.codes.page + h * c.codes.head + (32 * wv + col) * (PK6 ? 48 : 64);
         const int64_t meta = kp * c.meta.page + h * c.meta.head;
-        const uint32_t angles = (1u << c.tbits) - 1u;
+        // A pair's radius and angle are a scaled code and a constant each; the lanes make them for a pair each, in turns, of the cosine (a quarter turn on) and the sine.
+        const uint32_t table = lds_addr(constants) + wv * 2048;
+        {
+            const float rs = lo2f<T>(c.rscale[meta + lane]), rm = lo2f<T>(c.rmn[meta + lane]), ts = lo2f<T>(c.tscale[meta + lane]) * kTurn, tm = lo2f<T>(c.tmn[meta + lane]) * kTurn;
+            const float a0 = __builtin_fmaf(ts, 0.5f, tm), r0 = __builtin_fmaf(rs, 0.5f, rm), rw = rs / static_cast<float>(1 << c.tbits);
+            *lds_ptr<lds_f4>(table + lane * 16) = float4_v{rw, r0, ts, a0 + 0.25f};
+            *lds_ptr<lds_f4>(table + 1024 + lane * 16) = float4_v{rw, r0, ts, a0};
+        }
+        const uint32_t angles4 = ((1u << c.tbits) - 1u) * 0x01010101u;
         uint32_t words[16];
         if constexpr (PK6) {
             u32x4_a w[3];
@@ -115,19 +124,15 @@ __global__ __launch_bounds__(256, 2) void paged_weights_kernel(PagedWeightArgs a
                 for (int j = 0; j < 4; j++) words[4 * i + j] = w[j];
             }
         }
-        const float quarter = hi ? 0.0f : 0.25f;                             // (a cosine is the sine a quarter turn on)
         static_for<16>([&](auto I) {
             constexpr int i = decltype(I)::value;
-            const uint2 wr = *reinterpret_cast<const uint2*>(c.rscale + meta + 4 * i), wm = *reinterpret_cast<const uint2*>(c.rmn + meta + 4 * i);
-            const uint2 wt = *reinterpret_cast<const uint2*>(c.tscale + meta + 4 * i), wn = *reinterpret_cast<const uint2*>(c.tmn + meta + 4 * i);
+            const uint32_t r4 = words[i] & ~angles4, t4 = words[i] & angles4;
             float v[4];
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                auto half = [&](const uint2& w) { return lo2f<T>(static_cast<uint16_t>((k < 2 ? w.x : w.y) >> (16 * (k & 1)))); };
-                const uint32_t code = (words[i] >> (8 * k)) & 0xffu;
-                const float r = __builtin_fmaf(static_cast<float>(code >> c.tbits) + 0.5f, half(wr), half(wm));
-                const float turns = __builtin_fmaf(static_cast<float>(code & angles) + 0.5f, half(wt), half(wn)) * kTurn + quarter;
-                v[k] = r * __builtin_amdgcn_sinf(turns);
+                const float4_v w = *lds_ptr<lds_f4>(table + hi * 1024 + (4 * i + k) * 16);
+                v[k] = __builtin_fmaf(static_cast<float>((r4 >> (8 * k)) & 0xffu), w.x, w.y) *
+                       __builtin_amdgcn_sinf(__builtin_fmaf(static_cast<float>((t4 >> (8 * k)) & 0xffu), w.z, w.w));
             }
             const uint32_t a0 = pack_pair<T>(v[0], v[1]), a1 = pack_pair<T>(v[2], v[3]);
             auto rest = [&](uint32_t w, float x, float y) {

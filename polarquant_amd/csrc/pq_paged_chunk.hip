@@ -33,10 +33,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_chunk_kernel(PagedAttnArg
     const int limit = s.past + token;                                        // last key this row sees
     const int wave_row = row0 + wv * 32 < rows - 1 ? row0 + wv * 32 : rows - 1, wave_end = wave_row + 31 < rows - 1 ? wave_row + 31 : rows - 1;
     const int wave_first = uniform(s.past + wave_row / rep), wave_last = uniform(s.past + wave_end / rep), last_limit = uniform(s.past + last_row / rep);
-    const int p0 = min(unit.slice * unit.per, pages), p1 = min(p0 + unit.per, pages);
-    const int it0 = 2 * p0;
+    int p0 = min(unit.slice * unit.per, pages);
+    const int p1 = min(p0 + unit.per, pages);
     int it1 = 2 * p1 < (s.kv + kChunkKeys - 1) / kChunkKeys ? 2 * p1 : (s.kv + kChunkKeys - 1) / kChunkKeys;
     if (const int seen = last_limit < 0 ? 0 : last_limit / kChunkKeys + 1; it1 > seen) it1 = seen;
+    if (a.mask && 2 * p0 < it1) p0 = uniform(first_unmasked(a.mask + b * a.mask_row, p0 * kPageTokens, min(it1 * kChunkKeys, s.kv)) / kPageTokens);
+    const int it0 = 2 * p0;
     const int border = 2 * s.sealed;                                         // tiles from here on are open
 
     // ---- queries: in the order of a key's chunks of 16 bytes, of which this lane multiplies chunks 8 hi + i

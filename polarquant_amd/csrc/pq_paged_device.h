@@ -43,6 +43,28 @@ __device__ __forceinline__ int key_page(const PagedCache& c, const PagedSequence
 }
 __device__ __forceinline__ int value_page(const PagedCache& c, int b, int p) { return page_of(c.value_pages, c.values.n, static_cast<int64_t>(b) * c.W + p); }
 
+// Of a sequence's mask from key `from` on: the first 64 keys, counted from there, in which one is; or `to`.  Left padding is passed over before the pipelines start, which would
+// make its keys.
+__device__ __forceinline__ int first_unmasked(const uint8_t* mask, int from, int to) {
+    const int lane = threadIdx.x & 63;
+    for (; from < to; from += 16 * kWave) {
+        uint8_t byte[16];
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const int key = from + j * kWave + lane;
+            byte[j] = mask[key < to ? key : to - 1];
+        }
+        uint32_t any = 0;
+#pragma unroll
+        for (int j = 0; j < 16; j++) any |= __ballot(byte[j] != 0) ? 1u << j : 0u;
+        if (any) {
+            from += kWave * __builtin_ctz(any);
+            return from < to ? from : to;
+        }
+    }
+    return to;
+}
+
 // A workgroup's share: a row tile of a sequence and a slice of its pages.
 struct PagedUnit {
     int b, tile, slice, slices, per;          // per: pages a slice

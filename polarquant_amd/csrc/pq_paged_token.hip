@@ -76,10 +76,13 @@ __global__ __launch_bounds__(256, 2) void paged_token_kernel(PagedAttnArgs a) {
     int blocks = (s.kv + kTokenBlock - 1) / kTokenBlock;
     const int p0 = min(unit.slice * unit.per, pages), p1 = min(p0 + unit.per, pages);
     const int mine = p1 - p0;                 // (a quarter of four blocks a page)
-    const int blk0 = 4 * p0 + wv * mine;
+    int blk0 = 4 * p0 + wv * mine;
     const int seen = last_limit < 0 ? 0 : last_limit / kTokenBlock + 1;
     if (blocks > seen) blocks = seen;
     const int blk1 = blk0 + mine < blocks ? blk0 + mine : blocks;
+    if constexpr (MASK) {
+        if (blk0 < blk1) blk0 = uniform(first_unmasked(a.mask + b * a.mask_row, blk0 * kTokenBlock, min(blk1 * kTokenBlock, s.kv)) / kTokenBlock);
+    }
     const int border = 4 * s.sealed;
 
     floatx4_a o[NQ][8];

@@ -29,8 +29,8 @@
  * pq_paged_attn: out[t, h] = sum_j w_j v_j / sum_j w_j, w_j = exp(scale q . k_j), over the keys j of the sequence up to
  *   the token's own whose page exists and whose mask[b * mask_row + j] is not 0; zeros where there are none.  lse (or
  *   null): [T, N] natural logarithm of the sum, -inf where there are none.  The pages of all sequences are
- *   dealt out to `units` workgroups a KV head (pq_paged_attn_plan; at least one for every 16 or 128 rows of every sequence)
- *   by the lengths on the device, and joined through `workspace`; 0: no sequence is cut.
+ *   dealt out to `units` workgroups a KV head (pq_paged_attn_plan; at least one for every tile of 16, 128 or 256
+ *   rows that max_q rows of B sequences make) by the lengths on the device, and joined through `workspace`; 0: no sequence is cut.
  * pq_paged_weights: weights[b, g, j] = onto[b, g, j] (null: 0) + sum over the rows, the query heads of KV head g and the
  *   keys of page j that the row sees of exp(scale q . k - lse).  (No values are read: their page exists if it is not
  *   negative.)

@@ -12,6 +12,14 @@
 // Angles go through a table of cos and sin in LDS, 64 pairs x 16 bins of float16, which a wavefront makes once a page: word (pair % 16) 64 +
 // (pair / 16) 16 + bin, so that the lanes of a lookup, four pairs and sixteen keys, meet a bank only with a lane that wants the same word.
 // (More than 16 bins: cos and sin are evaluated for every code.)  Radii are (code + 1/2) (width of a bin) + (least).
+//
+// Rounded to 16 bits: cos and sin (the table's reads are what LDS has time for), a key's products with its radius and the weights (operands of the matrix cores; keys float16
+// for bfloat16 models too, scaled by a page's power of two).  Against 64 bits, 16 x 32 K: 1.3e-3 of the output in float16, where attention over keys in 32 bits has 2e-4;
+// in bfloat16 2.0e-3 and 1.7e-3.  Maxima, sums and the states that are joined: float32.
+//
+// What bounds it: memory.  16 x 32 K tokens, 32 heads over 8: 1.36 GB in 217 us, 6.3 TB/s; a ragged batch of 64, 363 MB in 72 us, 5.0 TB/s; one sequence of 2 K: 8 us, three
+// dependent trips to memory (lengths, tables, codes) and the join, and 4 for the merge.  Keys and values by way of LDS took 247 us in place of 231, row tiles not dealt
+// out over the device by lengths 87 us in place of 74 for the ragged batch; 32 rows a workgroup do not fit the registers.
 #include "pq_paged_device.h"
 
 namespace pq {

@@ -8,8 +8,9 @@ constexpr int kPagedFewRows = 16;             // rows a sequence that the kernel
 constexpr int kPagedMostRows = 256;           // rows of the largest tile
 
 // Rows of a workgroup of the kernel that a call of `rows` rows a sequence runs.  A tile of 256 rows makes its keys for twice as many rows as one of 128, but half as
-// many workgroups share the work.  With 32 heads over 8, 256 and 128 rows: 1273 and 1393 us for 2 K tokens behind 32 K, 121 and 131 for 512 behind 8 K, 707 and
-// 751 for eight such sequences, 279 and 295 for eight of up to that length; but 23 and 21 for 100 behind 1000, and 152 and 144 for 2 K behind 2 K.
+// many workgroups share the work.  With 32 heads over 8, 256 and 128 rows (before a tile's codes were asked for earlier): 1273 and 1393 us for 2 K tokens behind 32 K, 121
+// and 131 for 512 behind 8 K, 707 and 751 for eight such sequences, 279 and 295 for eight of up to that length; but 23 and 21 for 100 behind 1000, and 152 and 144 for 2 K
+// behind 2 K.
 inline int paged_tile_rows(int64_t rows, int64_t max_kv) { return rows <= kPagedFewRows ? 16 : rows <= 128 || max_kv <= 4096 ? 128 : kPagedMostRows; }
 
 inline int64_t paged_tiles(int B, int N, int Nk, int max_q, int max_kv) {

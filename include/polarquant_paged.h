@@ -19,7 +19,7 @@
  * A physical page outside of its pool (-1, say) does not exist: its tokens are not attended to, nothing is written.
  * The call's tokens are the last of their sequences, packed: sequence b's are rows q_start[b] .. q_start[b + 1] - 1 of T,
  * at most max_q of them, and it holds kv_len[b] <= max_kv tokens with them.  These counts live on the device; larger ones
- * are cut to max_q and max_kv (max_kv <= 128 W).  Rows from q_start[B] on are neither read nor written.
+ * are cut to max_q (a sequence's first rows) and max_kv (max_kv <= 128 W).  Rows from q_start[B] on are neither read nor written.
  *
  * pq_paged_append: q, k, v rows [T, heads * 128] (row strides multiples of 8), each query and key normed over its 128
  *   channels where q_norm, k_norm [128] are given (x * rsqrt(mean x^2 + eps) * w), then rotated by row positions[t] (null:

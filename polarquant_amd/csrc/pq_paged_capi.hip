@@ -55,7 +55,7 @@ int check_mask(const uint8_t* mask, int64_t mask_row, int B, int max_kv) {
 
 pq::PagedCache cache(const void* keys, const void* values, const uint8_t* codes, const void* rscale, const void* rmn, const void* tscale, const void* tmn,
                      const int64_t* layout, const int32_t* q_start, const int32_t* kv_len, const int32_t* n_sealed, const int32_t* pages,
-                     const int32_t* value_pages, const int32_t* open_pages, int W, int Wo, int T, int B, int N, int Nk, int max_kv, int rbits, int tbits) {
+                     const int32_t* value_pages, const int32_t* open_pages, int W, int Wo, int T, int B, int N, int Nk, int max_q, int max_kv, int rbits, int tbits) {
     pq::PagedCache c{};
     c.keys = {keys, layout[0], layout[1], static_cast<int>(layout[8])};
     c.values = {values, layout[2], layout[3], static_cast<int>(layout[9])};
@@ -71,7 +71,7 @@ pq::PagedCache cache(const void* keys, const void* values, const uint8_t* codes,
     c.pages = pages ? pages : value_pages;
     c.value_pages = value_pages;
     c.open_pages = open_pages;
-    c.W = W; c.Wo = Wo; c.T = T; c.B = B; c.N = N; c.Nk = Nk; c.max_kv = max_kv; c.rbits = rbits; c.tbits = tbits;
+    c.W = W; c.Wo = Wo; c.T = T; c.B = B; c.N = N; c.Nk = Nk; c.max_q = max_q; c.max_kv = max_kv; c.rbits = rbits; c.tbits = tbits;
     return c;
 }
 
@@ -106,7 +106,7 @@ int pq_paged_append(const void* q, int64_t q_row, const void* k, int64_t k_row, 
         return rc;
     pq::PagedAppendArgs a{};
     a.c = cache(keys, values, nullptr, nullptr, nullptr, nullptr, nullptr, layout, q_start, kv_len, n_sealed, nullptr, value_pages, open_pages, W, Wo, T, B, N, Nk,
-                max_kv, 4, 4);
+                max_q, max_kv, 4, 4);
     a.q = static_cast<const uint16_t*>(q); a.k = static_cast<const uint16_t*>(k); a.v = static_cast<const uint16_t*>(v);
     a.q_row = q_row; a.k_row = k_row; a.v_row = v_row;
     a.cos = static_cast<const uint16_t*>(cos); a.sin = static_cast<const uint16_t*>(sin);
@@ -162,7 +162,7 @@ int pq_paged_attn(const void* q, int64_t q_row, const void* keys, const void* va
         return rc;
     pq::PagedAttnArgs a{};
     a.c = cache(keys, values, codes, rscale, rmn, tscale, tmn, layout, q_start, kv_len, n_sealed, pages, value_pages, open_pages, W, Wo, T, B, N, Nk,
-                max_kv, rbits, tbits);
+                max_q, max_kv, rbits, tbits);
     a.q = static_cast<const uint16_t*>(q);
     a.q_row = q_row;
     a.mask = mask;
@@ -205,7 +205,7 @@ int pq_paged_weights(const void* q, int64_t q_row, const float* lse, const void*
         return rc;
     pq::PagedWeightArgs a{};
     a.c = cache(keys, nullptr, codes, rscale, rmn, tscale, tmn, layout, q_start, kv_len, n_sealed, pages, value_pages, open_pages, W, Wo, T, B, N, Nk,
-                max_kv, rbits, tbits);
+                max_q, max_kv, rbits, tbits);
     a.q = static_cast<const uint16_t*>(q);
     a.q_row = q_row;
     a.mask = mask;

@@ -19,7 +19,7 @@ __device__ __forceinline__ int within(int v, int lo, int hi) { return v < lo ? l
 __device__ __forceinline__ PagedSequence paged_sequence(const PagedCache& c, int b) {
     PagedSequence s;
     s.first = within(c.q_start[b], 0, c.T);
-    s.rows = within(c.q_start[b + 1], s.first, c.T) - s.first;
+    s.rows = within(within(c.q_start[b + 1], s.first, c.T) - s.first, 0, c.max_q);
     s.kv = within(c.kv_len[b], 0, c.max_kv);
     s.past = s.kv - s.rows;
     s.sealed = c.n_sealed ? within(c.n_sealed[b], 0, s.kv / kPageTokens) : 0;

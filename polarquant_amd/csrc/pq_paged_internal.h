@@ -21,7 +21,7 @@ struct PagedCache {
     const uint16_t *rscale, *rmn, *tscale, *tmn;
     const int32_t *q_start, *kv_len, *n_sealed;          // [B + 1], [B], [B] (null: none is sealed)
     const int32_t *pages, *value_pages, *open_pages;     // [B, W], [B, W], [B, Wo]
-    int W, Wo, T, B, N, Nk, max_kv, rbits, tbits;
+    int W, Wo, T, B, N, Nk, max_q, max_kv, rbits, tbits;
 };
 
 struct PagedAttnArgs {

@@ -447,7 +447,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a, int t
     const int b = blockIdx.y, lane = threadIdx.x & 63, rep = c.N / c.Nk;
     const PagedPartials part = paged_partials(a.partial, a.units, c.Nk, tile_rows);
     const int2 where = part.where[b];
-    const int first = within(c.q_start[b], 0, c.T), tokens = within(c.q_start[b + 1], first, c.T) - first;
+    const int first = within(c.q_start[b], 0, c.T), tokens = within(within(c.q_start[b + 1], first, c.T) - first, 0, c.max_q);
     const int i = static_cast<int>(blockIdx.x) * 4 + uniform(static_cast<int>(threadIdx.x >> 6)), token = i / c.N, head = i % c.N;
     if (token >= tokens || where.y <= 1) return;                             // (of one slice: written by it)
     const int h = head / rep, r = token * rep + head % rep, unit = where.x + r / tile_rows * where.y;

@@ -40,12 +40,13 @@ __global__ __launch_bounds__(256, 2) void paged_weights_kernel(PagedWeightArgs a
         return;
     }
     const uint32_t lds0 = lds_addr(sm);
-    // A row is a token and a query head, r / rep and r % rep.  From one tile to the next a lane's token goes on by 64 / rep, with its base, and its head by 64 % rep:
-    // nothing of it is left to the lanes where rep divides 64.
+    // A row is a token and a query head, r / rep and r % rep.  From one tile to the next the bases go on to the token of the tile's first row; a lane's place from there
+    // stays what it is where rep divides 64, and otherwise its head goes on by 64 % rep.
     const int step_t = kWeightRows / rep, step_head = kWeightRows % rep, t0 = tile0 * kWeightRows / rep;
     const uint32_t token_bytes = 2 * static_cast<uint32_t>(a.q_row);
     const uint16_t* base = a.q + (s.first + t0) * a.q_row + h * rep * 128;
     const float* lse_base = a.lse + (s.first + t0) * static_cast<int64_t>(c.N) + h * rep;
+    int base_head = tile0 * kWeightRows % rep;
     int head[6];                              // of this lane's four rows that it brings, and two whose scores it has
     uint32_t offset[6];                       // of their queries and log sums from the bases
     auto row_of = [&](int i) { return i < 4 ? (wv * 4 + i) * 4 + (lane >> 4) : 32 * (i - 4) + col; };
@@ -58,7 +59,7 @@ __global__ __launch_bounds__(256, 2) void paged_weights_kernel(PagedWeightArgs a
     float raw[2];                             // log sums of the rows of the tile that is on its way
     auto fetch = [&](int tile, int buf) __attribute__((always_inline)) {
         if ((tile + 1) * kWeightRows > rows) {                               // (the last row in place of those behind it)
-            const int t = s.rows - 1 - t0 - (tile - tile0) * step_t;
+            const int t = s.rows - 1 - tile * kWeightRows / rep;
             static_for<6>([&](auto I) {
                 if (tile * kWeightRows + row_of(I) >= rows) offset[I] = offset_of(I, t, rep - 1);
             });
@@ -74,11 +75,16 @@ __global__ __launch_bounds__(256, 2) void paged_weights_kernel(PagedWeightArgs a
         base += step_t * a.q_row;
         lse_base += step_t * static_cast<int64_t>(c.N);
         if (step_head) {
+            base_head += step_head;
+            const bool next = base_head >= rep;
+            base_head -= next ? rep : 0;
+            base += next ? a.q_row : 0;
+            lse_base += next ? c.N : 0;
             static_for<6>([&](auto I) {
                 head[I] += step_head;
                 const bool over = head[I] >= rep;
                 head[I] -= over ? rep : 0;
-                offset[I] += offset_of(I, 0, step_head) + (over ? offset_of(I, 1, 0) - offset_of(I, 0, rep) : 0u);
+                offset[I] += offset_of(I, 0, step_head) + (over ? offset_of(I, 1, 0) - offset_of(I, 0, rep) : 0u) - (next ? offset_of(I, 1, 0) : 0u);
             });
         }
     };

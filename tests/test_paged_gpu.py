@@ -153,6 +153,24 @@ def test_attention_reads_rows_as_they_lie_and_writes_no_others(gpu):
     assert got is out and bool((out[5:] == 7.0).all())
 
 
+@pytest.mark.parametrize("Nk,max_q,units", [(1, 3, 0), (1, 3, 5), (2, 20, 0), (2, 20, 40)])
+def test_more_new_tokens_than_max_q_are_cut(gpu, Nk, max_q, units):
+    """The first max_q rows of a sequence are its call's; the others are neither read nor written."""
+    c = Cache(gpu, [300, 200], [40, 2], [1, 0], 4, Nk, torch.bfloat16)
+    b = c.batch
+    few = PageBatch(b.q_start, b.kv_len, b.n_sealed, b.pages, b.open_pages, max_q, 300)
+    out = torch.full((c.T, 4, 128), 7.0, dtype=c.dtype, device=gpu)
+    q = c.q.clone()
+    q[max_q:40] = float("nan")
+    got, lse = paged_attention(q, c.pool, few, return_lse=True, units=units, out=out)
+    rows = list(range(max_q)) + [40, 41]
+    packed = PageBatch(torch.tensor([0, max_q, max_q + 2], dtype=torch.int32, device=gpu), b.kv_len, b.n_sealed, b.pages, b.open_pages, max_q, 300)
+    want, want_lse = paged_attention(c.q[rows].contiguous(), c.pool, packed, return_lse=True, units=units)
+    assert torch.equal(got[rows], want) and torch.equal(lse[rows], want_lse) and bool((out[max_q:40] == 7.0).all())
+    lse[max_q:40] = float("nan")
+    assert torch.equal(page_weights(q, lse, c.pool, few), page_weights(c.q[rows].contiguous(), want_lse, c.pool, packed))
+
+
 def test_attention_of_longer_contexts(gpu):
     """Many pages, so that every wavefront goes from page to page and the slices are dealt out unevenly."""
     c = Cache(gpu, [9000, 700, 4111], [1, 1, 1], [70, 5, 32], 28, 4, torch.bfloat16)
@@ -163,7 +181,7 @@ def test_attention_of_longer_contexts(gpu):
 
 # ---------------------------------------------------------------- weights
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("N,Nk,rbits,tbits,packed", [(4, 1, 4, 4, False), (14, 2, 3, 3, True), (8, 8, 4, 3, False), (40, 1, 1, 7, False)])
+@pytest.mark.parametrize("N,Nk,rbits,tbits,packed", [(4, 1, 4, 4, False), (14, 2, 3, 3, True), (8, 8, 4, 3, False), (40, 1, 1, 7, False), (70, 1, 4, 4, False)])
 def test_page_weights(gpu, dtype, N, Nk, rbits, tbits, packed):
     c = Cache(gpu, [1, 128, 300, 700, 0, 515], [1, 1, 33, 200, 0, 5], [0, 1, 1, 4, 0, 4], N, Nk, dtype, rbits, tbits, packed, wide=2)
     lse = c.attention()[2].float()

@@ -8,8 +8,8 @@
 // The sums are float32 and are held to that: a sealed key is split in two 16-bit parts, whose products are both added (2^-22 of it left in float16, 2^-16
 // in bfloat16, at random over 128 keys and more).  cos and sin are evaluated once a code: a key's lane pair takes one half each.
 //
-// What bounds it: products twice over, and an exponential a score.  512 tokens behind 16 K, 32 heads over 8: 70 GFLOP (140 with both parts) in 130 us; the compute units are
-// busy for 100 us of them (1056 pages on 512 to 768 places do not end together) and the matrix cores for 55.  A token of eight sequences over 4 K: 14 us, in which four
+// What bounds it: products twice over, and an exponential a score.  512 tokens behind 16 K, 32 heads over 8: 70 GFLOP (140 with both parts) in 126 us; the compute units are
+// busy for 95 us of them (1056 pages on 512 to 768 places do not end together) and the matrix cores for 55.  A token of eight sequences over 4 K: 12 us, in which four
 // workgroups a compute unit make a page's keys each, from three dependent trips to memory.  Tried: a tile's exponentials between the next one's products (136 us at 229 registers,
 // 17 in place of 14 for the tokens), four workgroups a compute unit (157 us, registers spilled).
 #include "pq_paged_device.h"
@@ -175,36 +175,41 @@ __global__ __launch_bounds__(256, 2) void paged_weights_kernel(PagedWeightArgs a
             const int buf = (tile - tile0) & 1;
             const float log_sum[2] = {raw[0] * kLog2e, raw[1] * kLog2e};
             if (tile + 1 < tiles) fetch(tile + 1, buf ^ 1);
-            floatx16_a z[2];
+            auto part = [&](auto HALVES) __attribute__((always_inline)) {
+                constexpr int halves = decltype(HALVES)::value;
+                floatx16_a z[halves];
 #pragma unroll
-            for (int u = 0; u < 2; u++)
+                for (int u = 0; u < halves; u++)
 #pragma unroll
-                for (int j = 0; j < 16; j++) z[u][j] = 0.0f;
-            static_for<8>([&](auto I) {
-                constexpr int i = decltype(I)::value;
+                    for (int j = 0; j < 16; j++) z[u][j] = 0.0f;
+                static_for<8>([&](auto I) {
+                    constexpr int i = decltype(I)::value;
 #pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    const u32x4_a q = *lds_ptr<lds_u32x4>(lds0 + buf * kWeightTile + (32 * u + col) * 256 + ((8 * hi + i) ^ (col & 15)) * 16);
-                    z[u] = mma32<T>(kf[i], q, z[u]);
-                    if constexpr (products == 16) z[u] = mma32<T>(kl[i], q, z[u]);
-                }
-            });
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const int r = tile * kWeightRows + 32 * u + col;
-                if (bits != 0xffffffffu || tile < whole) {
-                    const int last = s.past + (r < rows ? r : rows - 1) / rep - key0 - 4 * hi;
-                    const uint32_t there = bits >> (4 * hi);
-#pragma unroll
-                    for (int j = 0; j < 16; j++) {
-                        const int e = 8 * (j >> 2) + (j & 3);
-                        z[u][j] = e <= last && (there >> e & 1) ? z[u][j] : least;
+                    for (int u = 0; u < halves; u++) {
+                        const u32x4_a q = *lds_ptr<lds_u32x4>(lds0 + buf * kWeightTile + (32 * u + col) * 256 + ((8 * hi + i) ^ (col & 15)) * 16);
+                        z[u] = mma32<T>(kf[i], q, z[u]);
+                        if constexpr (products == 16) z[u] = mma32<T>(kl[i], q, z[u]);
                     }
-                }
-                const float sum2 = r < rows && log_sum[u] != -INFINITY ? log_sum[u] : INFINITY;
+                });
 #pragma unroll
-                for (int j = 0; j < 16; j++) total[j & 1] += exp2_hw(__builtin_fmaf(z[u][j], scale2, -sum2));
-            }
+                for (int u = 0; u < halves; u++) {
+                    const int r = tile * kWeightRows + 32 * u + col;
+                    if (bits != 0xffffffffu || tile < whole) {
+                        const int last = s.past + (r < rows ? r : rows - 1) / rep - key0 - 4 * hi;
+                        const uint32_t there = bits >> (4 * hi);
+#pragma unroll
+                        for (int j = 0; j < 16; j++) {
+                            const int e = 8 * (j >> 2) + (j & 3);
+                            z[u][j] = e <= last && (there >> e & 1) ? z[u][j] : least;
+                        }
+                    }
+                    const float sum2 = r < rows && log_sum[u] != -INFINITY ? log_sum[u] : INFINITY;
+#pragma unroll
+                    for (int j = 0; j < 16; j++) total[j & 1] += exp2_hw(__builtin_fmaf(z[u][j], scale2, -sum2));
+                }
+            };
+            if (rows - tile * kWeightRows > 32) part(IC<2>{});
+            else part(IC<1>{});               // (a token's few heads: half of it; 13.5 us -> 12.2 for eight sequences of 4 K)
             rows_arrived();
             __syncthreads();
         }

@@ -75,6 +75,20 @@ def test_attention_masks(gpu, new):
         assert torch.equal(paged_attention(c.q, c.pool, c.batch, attention_mask=other), out)
 
 
+@pytest.mark.parametrize("new", [[1, 1, 1, 1], [40, 1, 3, 2], [200, 7, 9, 1]])
+@pytest.mark.parametrize("units", [None, 0, 64])
+def test_attention_behind_long_left_padding(gpu, units, new):
+    """Padding over many pages, to the last key, from a page's middle, and of everything; what lies under it is not a number."""
+    c = Cache(gpu, [4300, 2049, 3000, 1500], new, [30, 16, 22, 11], 8, 2, torch.float16, seed=7)
+    c.mask = torch.ones(4, 4352, dtype=torch.uint8, device=gpu)
+    for b, n in enumerate([2500, 2048, 1100, 1500]):
+        c.mask[b, :n] = 0
+        for j in range(n // PAGE):
+            c.pool.values[c.pages[b, j].item()] = float("nan")
+    out, _ = check_attention(c, units=units)
+    assert bool((out[c.q_start[3]:] == 0).all())
+
+
 @pytest.mark.parametrize("new", [[1, 1], [50, 3]])
 def test_attention_passes_over_pages_that_do_not_exist(gpu, new):
     c = Cache(gpu, [700, 400], new, [4, 2], 8, 2, torch.float16)

@@ -9,7 +9,7 @@
 // in bfloat16, at random over 128 keys and more).  cos and sin are evaluated once a code: a key's lane pair takes one half each.
 //
 // What bounds it: products twice over, and an exponential a score.  512 tokens behind 16 K, 32 heads over 8: 70 GFLOP (140 with both parts) in 126 us; the compute units are
-// busy for 95 us of them (1056 pages on 512 to 768 places do not end together) and the matrix cores for 55.  A token of eight sequences over 4 K: 12 us, in which four
+// busy for 100 us of them (1056 pages on 512 to 768 places do not end together) and the matrix cores for 55.  A token of eight sequences over 4 K: 12 us, in which four
 // workgroups a compute unit make a page's keys each, from three dependent trips to memory.  Tried: a tile's exponentials between the next one's products (136 us at 229 registers,
 // 17 in place of 14 for the tokens), four workgroups a compute unit (157 us, registers spilled).
 #include "pq_paged_device.h"

@@ -15,7 +15,7 @@
 //
 // Rounded to 16 bits: cos and sin (the table's reads are what LDS has time for), a key's products with its radius and the weights (operands of the matrix cores; keys float16
 // for bfloat16 models too, scaled by a page's power of two).  Against 64 bits, 16 x 32 K: 1.3e-3 of the output in float16, where attention over keys in 32 bits has 2e-4;
-// in bfloat16 2.0e-3 and 1.7e-3.  Maxima, sums and the states that are joined: float32.
+// in bfloat16 2.0e-3 and 1.7e-3.  (cos and sin in 32 bits: 1.0e-3 in float16, for 2 % more time at 16 x 32 K and 4 % in the ragged batch.)  Maxima, sums and the states that are joined: float32.
 //
 // What bounds it: memory.  16 x 32 K tokens, 32 heads over 8: 1.36 GB in 217 us, 6.3 TB/s; a ragged batch of 64, 363 MB in 72 us, 5.0 TB/s; one sequence of 2 K: 8 us, three
 // dependent trips to memory (lengths, tables, codes) and the join, and 4 for the merge.  Keys and values by way of LDS took 247 us in place of 231, row tiles not dealt
